@@ -82,7 +82,7 @@ def draw(rng):
     def size(lo, hi):                      # spread over the logarithm
         return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
 
-    kw = dict(page=rng.choice([16, 32, 64, 64, 128]), lens=rng.randrange(1 << 20))
+    kw = dict(page=rng.choice([16, 32, 64, 64]), lens=rng.randrange(1 << 20))
     kind = rng.choice(["plan", "append", "append", "decode", "decode", "decode", "verify", "verify", "prefill", "prefill", "prefill"])
     if kind == "plan":
         if rng.random() < 0.5:
