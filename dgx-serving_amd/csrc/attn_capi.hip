@@ -2,6 +2,7 @@
 // include/dgx_attn.h. Host code only; every call returns a hipError_t and never aborts or exits.
 #include "attn_device.h"
 #include "attn_internal.h"
+#include "attn_kv8.h"
 #include "../../include/dgx_attn.h"
 #include <climits>
 #include <atomic>
@@ -333,6 +334,26 @@ bool f32_take_fast(const Problem &p, const Pool *&pool) {
     return f32_reserved(p, *pl);
 }
 
+// ---------------------------------------------------------------- paged 8-bit cache
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool kv8_page_ok(int page) { return page == 16 || page == 32 || page == 64; }
+bool kv8_cache_ok(const dgx_kv8 *c, Kv8 &k) {
+    if (!c || !c->K || !c->V || !c->Ks || !c->Vs || c->pages <= 0 || !kv8_page_ok(c->page) || c->NKV <= 0 || c->NKV > 65535 ||
+        !valid_hd(c->HD) || c->pages > INT_MAX / c->page || !aligned16(c->K) || !aligned16(c->V))
+        return false;
+    k = Kv8{static_cast<uint8_t *>(c->K), static_cast<uint8_t *>(c->V), c->Ks, c->Vs, c->pages, c->page,
+            c->page == 16 ? 4 : c->page == 32 ? 5 : 6, c->NKV, c->HD};
+    return true;
+}
+constexpr int kKv8MaxPos = 1 << 30, kKv8MaxChunk = 1 << 20;
+bool kv8_sizes_ok(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk) {
+    return B >= 0 && T >= 0 && rows >= 0 && NQ > 0 && NQ <= 65535 && NKV > 0 && NQ % NKV == 0 && valid_hd(HD) && max_pos >= 0 &&
+           max_pos < kKv8MaxPos && chunk >= 0 && chunk <= kKv8MaxChunk && chunk % 64 == 0 && (long long)B * T <= INT_MAX &&
+           T <= kKv8MaxPos && (long long)T * (NQ / NKV) <= INT_MAX / 2;
+}
+// Bytes of the partials of a call: m and l [rows * NQ * ns], each rounded up to 256 bytes, then acc.
+size_t kv8_bytes(size_t partials, int HD) { return 2 * ((partials * 4 + 255) / 256 * 256) + partials * (size_t)HD * 4; }
+
 }  // namespace
 
 extern "C" {
@@ -656,6 +677,68 @@ hipError_t dgx_attn_prefill(const void *Q, int q_dtype, const void *Kc, const vo
                             int window) {
     return dgx_attn_prefill_ex(Q, q_dtype, Kc, Vc, kv_dtype, O, o_dtype, lse, nseq, Sq, NQ, NKV, HD, base_b, base,
                                kv_stride, max_pos, kv_split, st, scale, window, 0);
+}
+
+hipError_t dgx_kv8_plan(const int *ctx, const int *add, int B, int page, int *table, long table_stride, int table_cols,
+                        const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots, int rows,
+                        int *status, hipStream_t st) {
+    if (B < 0 || !kv8_page_ok(page) || table_cols < 0 || table_stride < table_cols || free_cap < 0 || rows < 0 || !free_in ||
+        !free_out || !cu || !status || (B && (!ctx || !add)) || (B && table_cols && !table) || (free_cap && !free_pages) || (rows && !slots))
+        return hipErrorInvalidValue;
+    return launch_kv8_plan(ctx, add, B, page == 16 ? 4 : page == 32 ? 5 : 6, table, table_stride, table_cols, free_pages, free_cap,
+                           free_in, free_out, cu, slots, rows, status, st);
+}
+
+hipError_t dgx_kv8_append(const void *k_src, const void *v_src, int src_dtype, long k_stride, long v_stride, const dgx_kv8 *cache,
+                          const int *slots, int rows, hipStream_t st) {
+    Kv8 c;
+    if (!kv8_cache_ok(cache, c) || rows < 0 || !valid_dtype(src_dtype)) return hipErrorInvalidValue;
+    if (rows == 0) return hipSuccess;
+    const long row = (long)c.NKV * c.HD, per16 = src_dtype == DT_FP32 ? 4 : 8;
+    if (!k_src || !v_src || !slots || k_stride < row || v_stride < row || k_stride % per16 || v_stride % per16 || !aligned16(k_src) ||
+        !aligned16(v_src))
+        return hipErrorInvalidValue;
+    unsigned *stats = nullptr;
+    if (knob_on("G4_KV_STATS")) {
+        const hipError_t e = kv_stats_address(stats);
+        if (e != hipSuccess) return e;
+    }
+    return launch_kv8_append(k_src, v_src, src_dtype, k_stride, v_stride, c, slots, rows, stats, st);
+}
+
+size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree) {
+    if (!kv8_sizes_ok(B, T, rows, NQ, NKV, HD, max_pos, chunk)) return (size_t)-1;
+    if (B == 0 || T == 0 || rows == 0) return 0;
+    const Kv8Plan pl = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window < 0 ? 0 : window, tree != 0);
+    return pl.ns > 1 ? kv8_bytes((size_t)rows * NQ * pl.ns, HD) : 0;
+}
+
+hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,
+                        float *lse, int B, int T, int rows, int NQ, const int *ctx, const int *cu, const unsigned *anc, int max_pos,
+                        int chunk, void *ws, size_t ws_bytes, hipStream_t st, float scale, int window) {
+    Kv8 c;
+    if (!kv8_cache_ok(cache, c) || !kv8_sizes_ok(B, T, rows, NQ, c.NKV, c.HD, max_pos, chunk) ||
+        (q_dtype != DT_F16 && q_dtype != DT_BF16) || !valid_dtype(o_dtype))
+        return hipErrorInvalidValue;
+    if (B == 0 || T == 0 || rows == 0) return hipSuccess;
+    if (!Q || !O || !ctx || !table || !aligned16(Q) || !aligned16(O) || !aligned16(ws) || table_stride < max_pos / c.page + 1 ||
+        (!cu && rows != B * T) || (anc && T > 32))
+        return hipErrorInvalidValue;
+    if (window < 0) window = 0;
+    const Kv8Problem p{c, Q, q_dtype, O, o_dtype, lse, B, T, rows, NQ, ctx, cu, table, table_stride,
+                       reinterpret_cast<const uint32_t *>(anc), max_pos, resolve_scale(scale, c.HD), window};
+    const Kv8Plan pl = kv8_choose(B, T, rows, NQ, c.NKV, c.HD, max_pos, chunk, window, anc != nullptr);
+    Kv8Partials part{nullptr, nullptr, nullptr, pl.ns, pl.C};
+    if (pl.ns > 1) {
+        const size_t n = (size_t)rows * NQ * pl.ns, one = (n * 4 + 255) / 256 * 256;
+        if (!ws || ws_bytes < kv8_bytes(n, c.HD)) return hipErrorInvalidValue;
+        part.m = static_cast<float *>(ws);
+        part.l = reinterpret_cast<float *>(static_cast<char *>(ws) + one);
+        part.acc = reinterpret_cast<float *>(static_cast<char *>(ws) + 2 * one);
+    }
+    const hipError_t e = timed_launch(st, [&] { return pl.prefill ? launch_kv8_prefill(p, part, st) : launch_kv8_decode(p, part, st); });
+    if (e != hipSuccess || pl.ns == 1) return e;
+    return launch_kv8_combine(p, part, st);
 }
 
 hipError_t dgx_attn_timing(int on) {

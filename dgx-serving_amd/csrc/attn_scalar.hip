@@ -243,6 +243,14 @@ hipError_t launch_kv_append(const float *ks, const float *vs, void *Kc, void *Vc
     return hipGetLastError();
 }
 
+// Address of the counters on the current device, for kernels of other files.
+hipError_t kv_stats_address(unsigned *&out) {
+    void *p = nullptr;
+    const hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(g_kv_stats));
+    out = static_cast<unsigned *>(p);
+    return e;
+}
+
 hipError_t read_kv_stats(unsigned out[4]) {
     return hipMemcpyFromSymbol(out, HIP_SYMBOL(g_kv_stats), sizeof(unsigned) * 4, 0, hipMemcpyDeviceToHost);
 }

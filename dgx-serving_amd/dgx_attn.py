@@ -55,6 +55,10 @@ def lib():
             "dgx_attn_batch_ex": ([P, I, P, P, P, P, I, P, I, P, P, I, I, I, I, I, I, P, I, L64, P, I, I, P, F, I, I], I),
             "dgx_attn_prefill_ex": ([P, I, P, P, I, P, I, P, I, I, I, I, I, P, I, L64, I, I, P, F, I, I], I),
             "dgx_attn_prefill": ([P, I, P, P, I, P, I, P, I, I, I, I, I, P, I, L64, I, I, P, F, I], I),
+            "dgx_kv8_plan": ([P, P, I, I, P, L64, I, P, I, P, P, P, P, I, P, P], I),
+            "dgx_kv8_append": ([P, P, I, L64, L64, P, P, I, P], I),
+            "dgx_attn_kv8": ([P, I, P, P, L64, P, I, P, I, I, I, I, P, P, P, I, I, P, S, P, F, I], I),
+            "dgx_attn_kv8_workspace": ([I, I, I, I, I, I, I, I, I, I], S),
             "dgx_attn_version": ([], ctypes.c_char_p),
             "dgx_attn_timing": ([I], I),
             "dgx_attn_timing_read": ([P, P], I),
@@ -247,6 +251,115 @@ def attn_prefill(Q, K, V, O, nseq, Sq, NQ, NKV, HD, base=0, base_b=None, kv_stri
     _ck(lib().dgx_attn_prefill(_ptr(Q), _DT[Q.dtype], _ptr(K), _ptr(V), kv_code(K), _ptr(O), _DT[O.dtype], _ptr(lse),
                                nseq, Sq, NQ, NKV, HD, _ptr(base_b), base, kv_stride, max_pos, kv_split, _stream(),
                                float(scale), window), "dgx_attn_prefill")
+
+
+# ------------------------------------------------------------------ paged 8-bit cache
+class _KV8(ctypes.Structure):
+    _fields_ = [("K", ctypes.c_void_p), ("V", ctypes.c_void_p), ("Ks", ctypes.c_void_p), ("Vs", ctypes.c_void_p),
+                ("pages", ctypes.c_int), ("page", ctypes.c_int), ("NKV", ctypes.c_int), ("HD", ctypes.c_int)]
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _i32(t, what, dev):
+    _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == dev, f"{what}: a contiguous int32 tensor on {dev} is wanted")
+    return t.data_ptr()
+
+
+class KV8Cache:
+    """A paged 8-bit KV cache (struct dgx_kv8) over torch tensors, which it keeps: K [pages, NKV, page, HD] and V [pages, NKV,
+    HD, page] as float8_e4m3fn, Ks and Vs [pages, NKV] fp32. KV8Cache.empty() allocates them."""
+
+    def __init__(self, K, V, Ks, Vs):
+        _need(K.dim() == 4 and V.dim() == 4 and tuple(V.shape) == (K.shape[0], K.shape[1], K.shape[3], K.shape[2]),
+              "KV8Cache: K [pages, NKV, page, HD] and V [pages, NKV, HD, page] are wanted")
+        _need(tuple(Ks.shape) == tuple(Vs.shape) == tuple(K.shape[:2]), "KV8Cache: Ks and Vs [pages, NKV] are wanted")
+        _need(K.dtype == V.dtype == torch.float8_e4m3fn and Ks.dtype == Vs.dtype == torch.float32,
+              "KV8Cache: float8_e4m3fn codes and fp32 scales are wanted")
+        _need(all(t.is_contiguous() and t.device == K.device for t in (K, V, Ks, Vs)), "KV8Cache: contiguous tensors of one device are wanted")
+        _need(K.shape[2] in (16, 32, 64) and K.shape[3] in (128, 256, 512), "KV8Cache: pages of 16, 32 or 64 tokens and head dims of 128, 256 or 512 are wanted")
+        self.K, self.V, self.Ks, self.Vs = K, V, Ks, Vs
+        self.pages, self.NKV, self.page, self.HD = K.shape
+        self.device = K.device
+        self._c = _KV8(K.data_ptr(), V.data_ptr(), Ks.data_ptr(), Vs.data_ptr(), self.pages, self.page, self.NKV, self.HD)
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, pages, page, NKV, HD, device="cuda"):
+        def codes(*shape):
+            return torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        return cls(codes(pages, NKV, page, HD), codes(pages, NKV, HD, page), torch.ones(pages, NKV, device=device),
+                   torch.ones(pages, NKV, device=device))
+
+
+def _on_device(dev, what):
+    _need(dev.type == "cuda" and dev.index == _get_device(), f"{what}: the tensors are on {dev}, which is not the current device")
+
+
+def kv8_plan(ctx, add, page, table, free_pages, free_in, free_out, cu, slots, status):
+    """Block tables and slot maps of a step (dgx_kv8_plan): ctx, add [B], table [B, cols] (rows may be strided), free_pages
+    [cap], free_in / free_out / status [1], cu [B + 1], slots [rows], all int32. status tells whether the step took its
+    pages; nothing is checked on the host."""
+    dev, B = ctx.device, ctx.shape[0]
+    _on_device(dev, "kv8_plan")
+    _need(table.dtype == torch.int32 and table.dim() == 2 and table.device == dev and table.shape[0] == B and
+          (table.stride(1) == 1 or table.shape[1] <= 1), "kv8_plan: table [B, cols] int32 with contiguous rows is wanted")
+    _need(add.shape[0] == B and cu.shape[0] == B + 1 and ctx.dim() == add.dim() == cu.dim() == 1, "kv8_plan: ctx and add [B], cu [B + 1] are wanted")
+    _need(free_in.numel() >= 1 and free_out.numel() >= 1 and status.numel() >= 1, "kv8_plan: free_in, free_out and status hold one number each")
+    stride = table.stride(0) if B > 1 else table.shape[1]
+    _need(stride >= table.shape[1], "kv8_plan: the rows of table overlap")
+    _ck(lib().dgx_kv8_plan(_i32(ctx, "ctx", dev), _i32(add, "add", dev), B, page, table.data_ptr(), stride, table.shape[1],
+                           _i32(free_pages, "free_pages", dev), free_pages.numel(), _i32(free_in, "free_in", dev),
+                           _i32(free_out, "free_out", dev), _i32(cu, "cu", dev), _i32(slots, "slots", dev), slots.numel(),
+                           _i32(status, "status", dev), _stream()), "dgx_kv8_plan")
+
+
+def kv8_append(k, v, cache, slots):
+    """Append rows k, v [rows, NKV, HD] (fp32, f16 or bf16; rows may be strided) at slots [rows] (dgx_kv8_append)."""
+    dev, rows = cache.device, slots.shape[0]
+    _on_device(dev, "kv8_append")
+    for t in (k, v):
+        _need(tuple(t.shape) == (rows, cache.NKV, cache.HD) and t.dtype == k.dtype and t.dtype in _DT and t.device == dev and
+              t.stride(2) == 1 and t.stride(1) == cache.HD, "kv8_append: k and v [rows, NKV, HD] of one type with contiguous rows are wanted")
+    row = cache.NKV * cache.HD
+    _ck(lib().dgx_kv8_append(k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0) if rows > 1 else row, v.stride(0) if rows > 1 else row,
+                             cache._p, _i32(slots, "slots", dev), rows, _stream()), "dgx_kv8_append")
+
+
+def attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk=0, window=0, tree=False):
+    """Bytes of attn_kv8's workspace for these sizes (dgx_attn_kv8_workspace)."""
+    n = lib().dgx_attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, 1 if tree else 0)
+    _need(n != ctypes.c_size_t(-1).value, "attn_kv8_workspace: sizes that dgx_attn_kv8 refuses")
+    return n
+
+
+def attn_kv8(Q, cache, table, ctx, O, T, max_pos, cu=None, anc=None, chunk=0, ws=None, scale=0.0, window=0, lse=None):
+    """Attention over the paged 8-bit cache (dgx_attn_kv8): Q, O [rows, NQ, HD], table [B, cols] and ctx [B] int32, cu [B + 1]
+    (None: T rows each), anc [rows] int32, ws a uint8 tensor of attn_kv8_workspace bytes (allocated here when None)."""
+    dev, B, rows, NQ = cache.device, ctx.shape[0], Q.shape[0], Q.shape[1]
+    _on_device(dev, "attn_kv8")
+    _need(Q.dim() == 3 and Q.shape[2] == cache.HD and Q.shape == O.shape and Q.is_contiguous() and O.is_contiguous() and
+          Q.device == dev and O.device == dev and Q.dtype in (torch.float16, torch.bfloat16) and O.dtype in _DT,
+          "attn_kv8: contiguous Q (f16, bf16) and O [rows, NQ, HD] on the cache's device are wanted")
+    _need(table.dtype == torch.int32 and table.dim() == 2 and table.device == dev and table.shape[0] == B and
+          (table.stride(1) == 1 or table.shape[1] <= 1), "attn_kv8: table [B, cols] int32 with contiguous rows is wanted")
+    _need(table.shape[1] > max_pos // cache.page, "attn_kv8: table has too few columns for max_pos")
+    _need(cu is None or cu.shape[0] == B + 1, "attn_kv8: cu [B + 1] is wanted")
+    _need(anc is None or anc.numel() == rows, "attn_kv8: anc [rows] is wanted")
+    _need(lse is None or (lse.numel() == rows * NQ and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev),
+          "attn_kv8: lse [rows, NQ] fp32 is wanted")
+    if ws is None:
+        ws = torch.empty(attn_kv8_workspace(B, T, rows, NQ, cache.NKV, cache.HD, max_pos, chunk, window, anc is not None),
+                         dtype=torch.uint8, device=dev)
+    _need(ws.is_contiguous() and ws.device == dev, "attn_kv8: a contiguous ws on the cache's device is wanted")
+    stride = table.stride(0) if B > 1 else table.shape[1]
+    _ck(lib().dgx_attn_kv8(Q.data_ptr(), _DT[Q.dtype], cache._p, table.data_ptr(), stride, O.data_ptr(), _DT[O.dtype], _ptr(lse),
+                           B, T, rows, NQ, _i32(ctx, "ctx", dev), None if cu is None else _i32(cu, "cu", dev),
+                           None if anc is None else _i32(anc, "anc", dev), max_pos, chunk, ws.data_ptr(),
+                           ws.numel() * ws.element_size(), _stream(), float(scale), window), "dgx_attn_kv8")
 
 
 def timing(on):

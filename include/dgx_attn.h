@@ -218,6 +218,65 @@ hipError_t dgx_attn_prefill_ex(const void *Q, int q_dtype, const void *Kc, const
                                int base, long kv_stride, int max_pos, int kv_split, hipStream_t st, float scale,
                                int window, int kv_cap);
 
+/* ---- paged 8-bit KV cache (no reference counterpart: the reference stores fp32, f16 or bf16 rows) ----
+ *
+ * K and V as OCP e4m3 codes in pages of 16, 32 or 64 tokens with a power-of-two scale for each (page, KV head), K and V
+ * apart: value = code * scale, scale = 2^e with the least e in [-40, 40] for which the page's largest magnitude is at most
+ * 448 * 2^e. (Half the bytes of a 16-bit cache to stream per decoded token; a stored value is off by at most half a step of
+ * e4m3, 2^-4 of it or 2^-10 of the scale.) Which pages a request's tokens are in stands in a block table: token j of
+ * request b is token j % page of page table[b * table_stride + j / page].
+ * All pointers but `cache` itself are device memory. No call allocates, synchronises or keeps state: all can be captured. */
+typedef struct dgx_kv8 {
+    void *K;          /* [pages][NKV][page][HD] codes, 16-byte aligned */
+    void *V;          /* [pages][NKV][HD][page] codes, 16-byte aligned */
+    float *Ks, *Vs;   /* [pages][NKV] scales */
+    int pages, page, NKV, HD;   /* HD 128, 256 or 512; pages * page < 2^31 */
+} dgx_kv8;
+
+/* Block tables and slot maps of a step, from the requests' lengths. Request b holds ctx[b] tokens and gets add[b] more (both
+ * >= 0). It keeps its ceil(ctx / page) pages and takes what it needs besides from the top of the stack free_pages
+ * [free_cap], whose count is free_in[0], in the order of the requests. Written: the new pages' entries of table, cu[B + 1]
+ * (first row of each request among the step's rows), slots[rows] (page id * page + token of each row; -1 behind the last),
+ * free_out[0] (the count left; may be free_in). The ids in the stack stay as they are.
+ * status[0] = 0, or a sum of 1: too few free pages, 2: a request needs more than table_cols pages, 4: more than `rows` new
+ * tokens, 8: a negative length or a count outside [0, free_cap]. Then the step takes nothing: table and count stay as they
+ * are, every slot is -1 and cu is zero (an append and an attention call over them do nothing).
+ * To give pages back, write their ids over free_pages[count ..] and raise the count. */
+hipError_t dgx_kv8_plan(const int *ctx, const int *add, int B, int page, int *table, long table_stride, int table_cols,
+                        const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots, int rows,
+                        int *status, hipStream_t st);
+
+/* Append rows r = 0 .. rows - 1 of k_src and v_src ([NKV, HD] each, fp32 / f16 / bf16, k_stride and v_stride elements between
+ * rows: multiples of 16 bytes, 16-byte aligned) at slots[r]; rows with a slot outside [0, pages * page) are skipped. Rows of
+ * one page follow each other, in ascending slots, in one call (as dgx_kv8_plan's slots do), and no page is written by two
+ * requests or two overlapping calls.
+ * The page's scale becomes the least that holds the new rows and is at least its own, unless the rows begin at the page's
+ * token 0; the codes of earlier tokens are rounded again when it grows (exact but for codes that become smaller than 2^-6
+ * scales). Tokens behind the new rows keep their bytes. A token with a non-finite value in a head gets NaN codes in that
+ * head's K and 0 for the values of V that are not finite: rows that attend it become NaN, others are not touched by it.
+ * Counts into dgx_kv_stats with G4_KV_STATS=1 (non-finite source values, largest stored magnitude). */
+hipError_t dgx_kv8_append(const void *k_src, const void *v_src, int src_dtype, long k_stride, long v_stride, const dgx_kv8 *cache,
+                          const int *slots, int rows, hipStream_t st);
+
+/* Attention over the cache: single tokens, drafts and draft trees, prompts. Row r in [cu[b], cu[b + 1]) of Q [rows, NQ, HD]
+ * (f16 or bf16), O (fp32, f16 or bf16) and lse (optional, [rows, NQ], natural log) is token r - cu[b] of request b, at
+ * position ctx[b] + r - cu[b]; cu null: T rows each (rows = B * T). T bounds the rows of a request, max_pos every position
+ * (both on the host). The rows' own K and V are in the cache already. A row attends the keys up to its position, from
+ * pos - window + 1 on with a window, and with anc (T <= 32; [rows]) those tokens i of its request's rows whose bit i of anc[r]
+ * is set. Keys on a page whose table entry lies outside [0, pages) are not attended, so the entries of pages that were given
+ * back behind a window may be -1. A row that attends nothing gets O = 0 and lse = -inf; rows outside every request keep
+ * what O and lse hold.
+ * chunk: keys of a split (a multiple of 64; 0: chosen from the sizes). ws: dgx_attn_kv8_workspace bytes for the same
+ * sizes, 16-byte aligned, used by this call alone until it has run (calls on other streams and other graphs take their
+ * own). Results do not depend on the other requests of a batch, but the choices made from B, T and max_pos do.
+ * hipErrorInvalidValue for sizes or types outside the above, or a workspace that is too small. */
+hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,
+                        float *lse, int B, int T, int rows, int NQ, const int *ctx, const int *cu, const unsigned *anc, int max_pos,
+                        int chunk, void *ws, size_t ws_bytes, hipStream_t st, float scale, int window);
+/* Bytes of ws for dgx_attn_kv8 with these sizes (tree: anc is given); grows with rows and max_pos / chunk. (size_t)-1 for
+ * sizes that the call refuses. */
+size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree);
+
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers). With timing on, the main
  * kernel of every decode/verify (split or streaming kernel, without the LSE combine) and every prefill launch is
  * bracketed by a HIP event pair on its launch stream, for up to 4096 launches. dgx_attn_timing_read waits for the
