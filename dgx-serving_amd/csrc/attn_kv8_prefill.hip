@@ -56,6 +56,11 @@ __device__ __forceinline__ void load_to_lds16(const void *src, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
+// LDS at a byte offset. (A pointer formed from an opaque offset is generic, and its loads go the slow flat way.)
+template <class T> __device__ __forceinline__ __attribute__((address_space(3))) T *lds_at(unsigned off) {
+    return (__attribute__((address_space(3))) T *)(uintptr_t)off;
+}
+
 template <int HD, int RB, bool F16, int OT>
 __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     using Cf = Kv8PrefCfg<HD, RB>;
@@ -123,7 +128,12 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
         }
     };
     Ids cur{0, 0, 0}, nxt{0, 0, 0};
-    if (s_lo <= s_hi) { cur = ids_of(s_lo); nxt = ids_of(min(s_lo + 1, s_hi)); issue(s_lo, cur); }
+    float ksn = 1.f, vsn = 1.f;                                        // scales of the lane's 16 keys, one step ahead
+    auto scales = [&](int id) {
+        const size_t cell = (size_t)safe(id) * kc.NKV + h;
+        ksn = kc.Ks[cell]; vsn = kc.Vs[cell];
+    };
+    if (s_lo <= s_hi) { cur = ids_of(s_lo); nxt = ids_of(min(s_lo + 1, s_hi)); issue(s_lo, cur); scales(cur.s); }
 
     // Rows of this wave: block rb holds rows lrow .. lrow + 15 of the tile; lane ln the row lrow + ln.
     u32x4 qop[RB][KS];
@@ -161,13 +171,13 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     const unsigned vaddr = Cf::HALF + (unsigned)ln * 64 + ((unsigned)(spiece ^ ((ln >> 2) & 3)) << 4) + 8 * (g & 1);
 
     for (int s = s_lo; s <= s_hi; s++) {
-        const size_t cell = (size_t)safe(cur.s) * kc.NKV + h;
-        const float ksc = kc.Ks[cell], vsc = kc.Vs[cell];
-        const bool ok = (unsigned)cur.s < (unsigned)kc.pages;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // stage s has landed, from every wave
         __syncthreads();
+        const float ksc = ksn, vsc = vsn;
+        const bool ok = (unsigned)cur.s < (unsigned)kc.pages;
         if (s < s_hi) {
             issue(s + 1, nxt);
+            scales(nxt.s);
             cur = nxt;
             nxt = ids_of(min(s + 2, s_hi));
         }
@@ -176,17 +186,25 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) any |= jw <= whi[rb] && jw + 31 >= wlo[rb];
         if (!any) continue;                                            // (wave-uniform; the barriers are above)
-        const unsigned char *sb = smem + (size_t)(s & 1) * Cf::STAGE;
         f32x4 st[2][RB];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) st[t][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // (opaque bases: the fragments' addresses are formed at their reads, not held across the loop)
+        unsigned ka = lds0 + kaddr + (unsigned)(s & 1) * Cf::STAGE, va = lds0 + vaddr + (unsigned)(s & 1) * Cf::STAGE;
+        asm volatile("" : "+v"(ka), "+v"(va));
+        u32x4 kw[2][2];
+        auto read_k = [&](int d) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) kw[d & 1][t] = *lds_at<u32x4>((ka ^ (64 * d)) + 4 * t * HD);
+        };
+        read_k(0);
 #pragma unroll
         for (int d = 0; d < DC; d++) {
-            u32x4 w[2];
-#pragma unroll
-            for (int t = 0; t < 2; t++) w[t] = *reinterpret_cast<const u32x4 *>(sb + ((kaddr + 4 * t * HD) ^ (64 * d)));
+            if (d + 1 < DC) read_k(d + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const u32x4 (&w)[2] = kw[d & 1];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const u32x4 k0 = e4m3_op<F16>(w[t][0], w[t][1]), k1 = e4m3_op<F16>(w[t][2], w[t][3]);
@@ -233,27 +251,41 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
             l[rb] = __builtin_fmaf(sum, iv, l[rb]);
             pf[rb] = u32x4{pack2<true>(tv[0], tv[1]), pack2<true>(tv[2], tv[3]), pack2<true>(tv[4], tv[5]), pack2<true>(tv[6], tv[7])};
         }
-        auto pv = [&](auto masked) {
-            u32x2 keep{0xffffffffu, 0xffffffffu};
-            if constexpr (decltype(masked)::value) {                   // bytes that are no token of the request's weigh nothing, NaN codes neither
-                const int k0 = ok ? max(j_lo - jw - 8 * g, 0) : 8, k1 = min(j_hi - jw - 8 * g, 8);
+        if (part) {
+            // Bytes that are no token of the request's weigh nothing, NaN codes neither: cleared in LDS, in the wave's own 32
+            // keys (the other row groups clear the same ones before they read them). Rare, and a mask in the loop below would
+            // cost 2 operations per fragment of 8, a second copy of the loop 64 registers.
+            const int k0 = ok ? max(j_lo - jw - 8 * g, 0) : 8, k1 = min(j_hi - jw - 8 * g, 8);
+            u32x2 keep;
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    const int x = min(max(k0 - 4 * w, 0), 4), y = min(max(k1 - 4 * w, 0), 4);
-                    keep[w] = (y >= 4 ? 0xffffffffu : (1u << (8 * y)) - 1u) & ~(x >= 4 ? 0xffffffffu : (1u << (8 * x)) - 1u);
-                }
+            for (int w = 0; w < 2; w++) {
+                const int x = min(max(k0 - 4 * w, 0), 4), y = min(max(k1 - 4 * w, 0), 4);
+                keep[w] = (y >= 4 ? 0xffffffffu : (1u << (8 * y)) - 1u) & ~(x >= 4 ? 0xffffffffu : (1u << (8 * x)) - 1u);
             }
-#pragma unroll
+#pragma unroll 1
             for (int d = 0; d < DB; d++) {
-                u32x2 w = *reinterpret_cast<const u32x2 *>(sb + vaddr + 1024 * d);
-                if constexpr (decltype(masked)::value) w &= keep;
-                const u32x4 v = e4m3_op<true>(w[0], w[1]);
-#pragma unroll
-                for (int rb = 0; rb < RB; rb++) acc[rb][d] = mfma16<true>(v, pf[rb], acc[rb][d]);
+                const u32x2 w = *lds_at<u32x2>(va + 1024 * d);
+                *lds_at<u32x2>(va + 1024 * d) = w & keep;
             }
+        }
+        constexpr int VB = 4;                                          // dim blocks read ahead
+        u32x2 vw[2][VB];
+        auto read_v = [&](int b) {
+#pragma unroll
+            for (int x = 0; x < VB; x++) vw[b & 1][x] = *lds_at<u32x2>(va + 1024 * (b * VB + x));
         };
-        if (part) pv(std::true_type{});
-        else pv(std::false_type{});
+        read_v(0);
+#pragma unroll
+        for (int b = 0; b < DB / VB; b++) {
+            if (b + 1 < DB / VB) read_v(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < VB; x++) {
+                const u32x4 v = e4m3_op<true>(vw[b & 1][x][0], vw[b & 1][x][1]);
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++) acc[rb][b * VB + x] = mfma16<true>(v, pf[rb], acc[rb][b * VB + x]);
+            }
+        }
     }
 
     // Merge of the two key groups: each wave finishes half of the dims of its rows and hands the other half over.
@@ -265,7 +297,16 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
         if (g == 0) { stm[(wave * RB + rb) * 16 + ln] = m[rb]; stl[(wave * RB + rb) * 16 + ln] = l[rb]; }
         float *x = xb + ((size_t)(wave * RB + rb) * 16 + ln) * Cf::XSTR + 4 * g;
 #pragma unroll
-        for (int d = 0; d < DB / 2; d++) *reinterpret_cast<f32x4 *>(x + 16 * d) = kg ? acc[rb][d] : acc[rb][DB / 2 + d];
+        for (int d = 0; d < DB / 2; d++) {
+            const f32x4 a0 = acc[rb][d], a1 = acc[rb][DB / 2 + d];     // (by value: a choice of addresses would put acc in memory)
+            f32x4 give;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                give[i] = kg ? a0[i] : a1[i];
+                acc[rb][d][i] = kg ? a1[i] : a0[i];                    // what it keeps
+            }
+            *reinterpret_cast<f32x4 *>(x + 16 * d) = give;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -284,7 +325,7 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
         const size_t px = row * a.part.ns + c;
 #pragma unroll
         for (int d = 0; d < DB / 2; d++) {
-            const f32x4 mine = kg ? acc[rb][DB / 2 + d] : acc[rb][d], other = *reinterpret_cast<const f32x4 *>(x + 16 * d);
+            const f32x4 mine = acc[rb][d], other = *reinterpret_cast<const f32x4 *>(x + 16 * d);
             f32x4 v = mine * f0 + other * f1;
             if (a.ns > 1) {
                 *reinterpret_cast<f32x4 *>(a.part.acc + px * HD + dim0 + 16 * d) = v;
