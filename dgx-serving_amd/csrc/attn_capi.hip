@@ -339,7 +339,7 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 bool kv8_page_ok(int page) { return page == 16 || page == 32 || page == 64; }
 bool kv8_cache_ok(const dgx_kv8 *c, Kv8 &k) {
     if (!c || !c->K || !c->V || !c->Ks || !c->Vs || c->pages <= 0 || !kv8_page_ok(c->page) || c->NKV <= 0 || c->NKV > 65535 ||
-        !valid_hd(c->HD) || c->pages > INT_MAX / c->page || !aligned16(c->K) || !aligned16(c->V))
+        !valid_hd(c->HD) || c->pages > INT_MAX / c->page || c->pages > INT_MAX / c->NKV || !aligned16(c->K) || !aligned16(c->V))
         return false;
     k = Kv8{static_cast<uint8_t *>(c->K), static_cast<uint8_t *>(c->V), c->Ks, c->Vs, c->pages, c->page,
             c->page == 16 ? 4 : c->page == 32 ? 5 : 6, c->NKV, c->HD};

@@ -83,6 +83,19 @@ struct Kv8Partials {
     int ns, C;                        // splits of a row at most, keys of a split (0: none, the kernel writes O itself)
 };
 
+// A value that is the same in all lanes and that no kernel of this library writes while this one runs, through the scalar
+// cache: page ids and scales then cost no vector registers and no wait behind the vector loads in flight.
+template <class T> __device__ __forceinline__ T scalar_load(const T *p) {
+    return *(const __attribute__((address_space(4))) T *)(uintptr_t)p;
+}
+
+// Four neighbouring dims of an output row, rounded once to the type of O.
+__device__ __forceinline__ void kv8_store4(const Kv8Problem &p, size_t at, const f32x4 &v) {
+    if (p.o_dtype == DT_FP32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.O) + at) = v;
+    else *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.O) + at) =
+        p.o_dtype == DT_F16 ? u32x2{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])} : u32x2{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])};
+}
+
 // Merge weight of a partial state (m, l) under the common reference M >= m. A state that saw no key has m = -inf and
 // l = 0; one whose only keys were NaN has m = -inf and l = NaN, which must reach the result.
 __device__ __forceinline__ float kv8_weight(float m, float l, float M) { return m == kNegInf ? l * 0.f : fast_exp2(m - M); }

@@ -61,7 +61,7 @@ template <class T> __device__ __forceinline__ __attribute__((address_space(3))) 
     return (__attribute__((address_space(3))) T *)(uintptr_t)off;
 }
 
-template <int HD, int RB, bool F16, int OT>
+template <int HD, int RB, bool F16>
 __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     using Cf = Kv8PrefCfg<HD, RB>;
     constexpr int DC = Cf::DC, DB = Cf::DB, KS = Cf::KS, NLD = Cf::NLD, SLOTS = Cf::SLOTS;
@@ -107,33 +107,59 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     const int page = kc.page, last_col = p.max_pos >> kc.lp;
     const int *tab = p.table + (size_t)seq * p.table_stride;
     auto safe = [&](int id) { return (unsigned)id < (unsigned)kc.pages ? id : 0; };
-    auto page_of = [&](int s, int piece) { return tab[min((64 * s + 16 * piece) >> kc.lp, last_col)]; };   // of a step's 16-key piece
+    // Pages of a step's four 16-key pieces, and the scales of the wave's two: all uniform, loaded a step or two ahead.
+    struct Ids { int p[4]; };
+    auto ids_of = [&](int s) {
+        Ids q;
+#pragma unroll
+        for (int i = 0; i < 4; i++) q.p[i] = scalar_load(tab + min((64 * s + 16 * i) >> kc.lp, last_col));
+        return q;
+    };
+    struct Scales { float k[2], v[2]; bool ok[2]; };
+    auto scales_of = [&](const Ids &q) {
+        Scales r;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int id = kg ? q.p[2 + i] : q.p[i];
+            const size_t cell = (size_t)safe(id) * kc.NKV + h;
+            r.ok[i] = (unsigned)id < (unsigned)kc.pages;
+            r.k[i] = scalar_load(kc.Ks + cell); r.v[i] = scalar_load(kc.Vs + cell);
+        }
+        return r;
+    };
 
     // Step loads. K slot S = (wave NLD + u) 64 + lane: key S / SLOTS, 16-byte column (S % SLOTS) ^ kf(key); a wave's keys lie
     // in one 16-key piece (wave / 2). V slot S: dim S / 4, piece (S % 4) ^ (dim / 4 % 4), which is the same in all u.
     auto kf = [](int key) { return HD == 128 ? ((key >> 1) & 1) | ((key >> 3) & 3) << 1 : (key & 3) | ((key >> 3) & 3) << 2; };
-    const int vpiece = (lane & 3) ^ ((lane >> 4) & 3), spiece = 2 * kg + (g >> 1);
-    struct Ids { int k, v, s; };                                       // pages: of the lane's K loads, V loads, scores
-    auto ids_of = [&](int s) { return Ids{page_of(s, wave >> 1), page_of(s, vpiece), page_of(s, spiece)}; };
+    const int vpiece = (lane & 3) ^ ((lane >> 4) & 3), kpiece = wave >> 1;
     const unsigned lds0 = (unsigned)(uintptr_t)smem;
+    unsigned koff[NLD];                                                // K: key in the piece's page rows, column
+#pragma unroll
+    for (int u = 0; u < NLD; u++) {
+        const int S = (wave * NLD + u) * 64 + lane, key = S / SLOTS;
+        koff[u] = (unsigned)((key & 15) * HD + (((S % SLOTS) ^ kf(key)) << 4));
+    }
+    const size_t head_bytes = (size_t)page * HD;
     auto issue = [&](int s, const Ids &q) {
         const unsigned st = lds0 + (unsigned)(s & 1) * Cf::STAGE + (unsigned)wave * NLD * 1024;
-        const uint8_t *kb = kc.K + ((size_t)safe(q.k) * kc.NKV + h) * ((size_t)page * HD);
-        const uint8_t *vb = kc.V + ((size_t)safe(q.v) * kc.NKV + h) * ((size_t)page * HD) + ((64 * s + 16 * vpiece) & (page - 1));
+        const int kid = safe(kpiece == 0 ? q.p[0] : kpiece == 1 ? q.p[1] : kpiece == 2 ? q.p[2] : q.p[3]);
+        const uint8_t *kb = kc.K + ((size_t)kid * kc.NKV + h) * head_bytes + (size_t)((64 * s + 16 * kpiece) & (page - 1)) * HD;
+        const int vid = vpiece < 2 ? (vpiece ? safe(q.p[1]) : safe(q.p[0])) : vpiece == 2 ? safe(q.p[2]) : safe(q.p[3]);
+        const uint8_t *vb = kc.V + ((size_t)(unsigned)(vid * kc.NKV + h)) * head_bytes + (unsigned)((wave * NLD * 16 + (lane >> 2)) * page + ((64 * s + 16 * vpiece) & (page - 1)));
 #pragma unroll
         for (int u = 0; u < NLD; u++) {
-            const int S = (wave * NLD + u) * 64 + lane, key = S / SLOTS, col = (S % SLOTS) ^ kf(key);
-            load_to_lds16(kb + (size_t)((64 * s + key) & (page - 1)) * HD + col * 16, st + u * 1024);
-            load_to_lds16(vb + (size_t)(S >> 2) * page, st + Cf::HALF + u * 1024);
+            load_to_lds16(kb + koff[u], st + u * 1024);
+            load_to_lds16(vb + 16 * u * page, st + Cf::HALF + u * 1024);
         }
     };
-    Ids cur{0, 0, 0}, nxt{0, 0, 0};
-    float ksn = 1.f, vsn = 1.f;                                        // scales of the lane's 16 keys, one step ahead
-    auto scales = [&](int id) {
-        const size_t cell = (size_t)safe(id) * kc.NKV + h;
-        ksn = kc.Ks[cell]; vsn = kc.Vs[cell];
-    };
-    if (s_lo <= s_hi) { cur = ids_of(s_lo); nxt = ids_of(min(s_lo + 1, s_hi)); issue(s_lo, cur); scales(cur.s); }
+    Ids nxt{{0, 0, 0, 0}};
+    Scales sn{{1.f, 1.f}, {1.f, 1.f}, {true, true}};
+    if (s_lo <= s_hi) {
+        const Ids q = ids_of(s_lo);
+        nxt = ids_of(min(s_lo + 1, s_hi));
+        issue(s_lo, q);
+        sn = scales_of(q);
+    }
 
     // Rows of this wave: block rb holds rows lrow .. lrow + 15 of the tile; lane ln the row lrow + ln.
     u32x4 qop[RB][KS];
@@ -168,17 +194,15 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     // or kg at HD 256 and 512 and not on t at 128 either.
     const int krow = 32 * kg + 8 * (ln >> 2) + (ln & 3);
     const unsigned kaddr = (unsigned)krow * HD + ((unsigned)(g ^ kf(krow)) << 4);
-    const unsigned vaddr = Cf::HALF + (unsigned)ln * 64 + ((unsigned)(spiece ^ ((ln >> 2) & 3)) << 4) + 8 * (g & 1);
+    const unsigned vaddr = Cf::HALF + (unsigned)ln * 64 + ((unsigned)((2 * kg + (g >> 1)) ^ ((ln >> 2) & 3)) << 4) + 8 * (g & 1);
 
     for (int s = s_lo; s <= s_hi; s++) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // stage s has landed, from every wave
         __syncthreads();
-        const float ksc = ksn, vsc = vsn;
-        const bool ok = (unsigned)cur.s < (unsigned)kc.pages;
+        const Scales sc = sn;
         if (s < s_hi) {
             issue(s + 1, nxt);
-            scales(nxt.s);
-            cur = nxt;
+            sn = scales_of(nxt);
             nxt = ids_of(min(s + 2, s_hi));
         }
         const int jw = 64 * s + 32 * kg;
@@ -214,9 +238,10 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
                 for (int rb = 0; rb < RB; rb++) st[t][rb] = mfma16<F16>(k1, qop[rb][2 * d + 1], st[t][rb]);
             }
         }
-        const int ve = exp_of(vsc);
-        const float f = ksc * a.sl2, ev = (float)ve, iv = pow2i(-ve);
-        const bool part = jw < j_lo || jw + 32 > j_hi || __any(!ok);
+        const bool up = g >= 2, ok = up ? sc.ok[1] : sc.ok[0];         // the lane's 8 keys are in piece g / 2 of the wave's
+        const float f = (up ? sc.k[1] : sc.k[0]) * a.sl2, ev = up ? (float)exp_of(sc.v[1]) : (float)exp_of(sc.v[0]);
+        const float iv = up ? pow2i(-exp_of(sc.v[1])) : pow2i(-exp_of(sc.v[0]));
+        const bool part = jw < j_lo || jw + 32 > j_hi || !(sc.ok[0] & sc.ok[1]);
         u32x4 pf[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
@@ -332,9 +357,7 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
                 continue;
             }
             v *= inv;
-            if constexpr (OT == DT_FP32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.O) + row * HD + dim0 + 16 * d) = v;
-            else *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.O) + row * HD + dim0 + 16 * d) =
-                u32x2{pack2<OT == DT_F16>(v[0], v[1]), pack2<OT == DT_F16>(v[2], v[3])};
+            kv8_store4(p, row * HD + dim0 + 16 * d, v);
         }
         if (kg == 0 && g == 0) {
             if (a.ns > 1) { a.part.m[px] = M; a.part.l[px] = L; }
@@ -343,7 +366,7 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     }
 }
 
-template <int HD, int RB, bool F16, int OT>
+template <int HD, int RB, bool F16>
 static hipError_t launch_pre_k(const Kv8PrefArgs &a, hipStream_t st) {
     using Cf = Kv8PrefCfg<HD, RB>;
     const long long G = a.p.NQ / a.p.c.NKV;
@@ -351,21 +374,14 @@ static hipError_t launch_pre_k(const Kv8PrefArgs &a, hipStream_t st) {
     const long long wgs = tiles * a.p.c.NKV * a.ns;
     if (wgs > INT_MAX) return hipErrorInvalidConfiguration;
     // (per device; setting it again changes nothing)
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv8_prefill_kernel<HD, RB, F16, OT>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv8_prefill_kernel<HD, RB, F16>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)Cf::LDS);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((kv8_prefill_kernel<HD, RB, F16, OT>), dim3((unsigned)wgs), dim3(512), Cf::LDS, st, a);
+    hipLaunchKernelGGL((kv8_prefill_kernel<HD, RB, F16>), dim3((unsigned)wgs), dim3(512), Cf::LDS, st, a);
     return hipGetLastError();
 }
-template <int HD, int RB, bool F16> static hipError_t launch_pre_o(const Kv8PrefArgs &a, hipStream_t st) {
-    switch (a.p.o_dtype) {
-    case DT_FP32: return launch_pre_k<HD, RB, F16, DT_FP32>(a, st);
-    case DT_F16: return launch_pre_k<HD, RB, F16, DT_F16>(a, st);
-    default: return launch_pre_k<HD, RB, F16, DT_BF16>(a, st);
-    }
-}
 template <int HD, int RB> static hipError_t launch_pre(const Kv8PrefArgs &a, hipStream_t st) {
-    return a.p.q_dtype == DT_F16 ? launch_pre_o<HD, RB, true>(a, st) : launch_pre_o<HD, RB, false>(a, st);
+    return a.p.q_dtype == DT_F16 ? launch_pre_k<HD, RB, true>(a, st) : launch_pre_k<HD, RB, false>(a, st);
 }
 
 hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st) {

@@ -230,7 +230,7 @@ typedef struct dgx_kv8 {
     void *K;          /* [pages][NKV][page][HD] codes, 16-byte aligned */
     void *V;          /* [pages][NKV][HD][page] codes, 16-byte aligned */
     float *Ks, *Vs;   /* [pages][NKV] scales */
-    int pages, page, NKV, HD;   /* HD 128, 256 or 512; pages * page < 2^31 */
+    int pages, page, NKV, HD;   /* HD 128, 256 or 512; pages * page and pages * NKV < 2^31 */
 } dgx_kv8;
 
 /* Block tables and slot maps of a step, from the requests' lengths. Request b holds ctx[b] tokens and gets add[b] more (both
