@@ -2,14 +2,18 @@
 // splits.
 //
 // A workgroup owns one key chunk of one request and KV head and up to 16 NT of its query rows (token-major: tokens x q-heads
-// of the KV head, so a byte of K or V is read once for the whole group). Its waves take the chunk's steps of 64 keys in turn
-// and run independent online softmaxes, merged at the end. Per step and wave everything goes from memory to the matrix
-// units through registers alone:
-//   * S^T = K Q^T on 16x16x32. Tile t (of 4) of a step holds the keys 16 (rho / 4) + 4 t + rho % 4 in its rows rho, so lane
-//     group g gets the scores of the 16 consecutive keys 16 g .. 16 g + 15 (4 t + i) of query row ln. A lane's 16-byte load
-//     is 16 dims of one key: two MFMA operands after the conversion to 16 bits, which is exact.
-//   * O^T += V^T P^T: V pages hold [dim][token], so a lane's 16-byte load is 16 consecutive tokens of one dim, the same 16
-//     keys whose probabilities the lane group holds. P never leaves its lane.
+// of the KV head, so a byte of K or V is read once for the whole group). It walks the chunk in steps of 128 keys at absolute
+// positions. Its NW waves split a step twice: each computes the scores of 16 KT of its keys against all rows, and, after the
+// probabilities went through LDS, the product of all 128 keys with HD / NW of V's dims. So
+//   * K and V go from memory to the matrix units through registers alone, and every code is loaded and converted to 16 bits
+//     (exactly) once per workgroup: half the accumulators per wave would be twice the conversions, and the other way round;
+//   * a wave holds 16 rows x HD / NW dims of the output (16 registers at HD 256 instead of the 64 of a wave that walks its
+//     own keys), which leaves registers for 3 to 4 waves per SIMD, and there is no merge of waves at the end;
+//   * the price is two barriers a step: for the row maxima, and for the probabilities.
+// S^T = K Q^T on 16x16x32: a lane's 16-byte load is 16 dims of one key, two operands. O^T += V^T P^T: V pages hold
+// [dim][token], so a lane's 16-byte load is 16 consecutive tokens of one dim, and its P operand is 16 neighbouring
+// probabilities of its row in LDS.
+//
 // The V scale 2^e of a key's page is part of its weight: P = 2^(s + e - m) multiplies the bare codes, with m the running
 // maximum of s + e, and the row sum takes P 2^-e. So P in f16 (11 bits) is as exact relative to the largest contribution
 // as it would be without scales, whatever the scales are. P is kept below 2^14 by holding the reference 2^6 under the
@@ -18,8 +22,8 @@
 // Chunks and steps lie at absolute keys and a step's wave depends on its position alone: a row's bits do not depend on the
 // other requests of the batch.
 //
-// What bounds it: HBM bytes of K and V. Conversions take 1/16 of the VALU's time at 6 TB/s (v_cvt_scalef32_pk_f16_fp8 issues
-// at full rate: 4.7 cycles measured, as an fma), MFMAs about a tenth of theirs.
+// What bounds it: HBM bytes of K and V. Conversions (v_cvt_scalef32_pk_f16_fp8 issues at full rate: 4.7 cycles measured, as
+// an fma) and MFMAs take about a tenth of their pipes' time at 6 TB/s.
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
@@ -70,25 +74,26 @@ __device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M,
 
 template <int HD, int NT>
 struct Kv8DecCfg {
-    static constexpr int NW = 4;                       // waves
+    static constexpr int SK = 128;                     // keys of a step
+    static constexpr int NW = HD == 512 ? 8 : 4;       // waves
+    static constexpr int KT = SK / 16 / NW;            // 16-key tiles of a wave
     static constexpr int RR = 16 * NT;                 // query rows
     static constexpr int DC = HD / 64;                 // 64-dim pieces of a key (one 16-byte load per lane each)
-    static constexpr int DB = HD / 16;                 // 16-dim output blocks
+    static constexpr int DB = HD / NW / 16;            // 16-dim output blocks of a wave
     static constexpr int QSTR = HD + 8;                // Q row in LDS: 16 rows on distinct bank quads
-    static constexpr int BSTR = HD + 4;
-    static constexpr size_t LDS_Q = (size_t)RR * QSTR * 2;
-    static constexpr size_t LDS_M = ((size_t)2 * NW * RR + (size_t)RR * BSTR) * 4;
-    static constexpr size_t LDS = LDS_Q > LDS_M ? LDS_Q : LDS_M;       // the merge reuses Q's place
-    // Two waves per SIMD where K, V and the accumulators of a wave fit 256 registers.
-    static constexpr int OCC = HD / 16 * 4 * NT + HD / 2 + 16 * NT <= 208 ? 2 : 1;
+    static constexpr int PSTR = SK + 8;                // P row, likewise
+    static constexpr size_t LDS_Q = (size_t)RR * QSTR * 2, LDS_P = (size_t)RR * PSTR * 2;
+    static constexpr size_t LDS = LDS_Q + LDS_P + (size_t)NW * RR * 4;
+    static constexpr int OCC = NT == 1 ? 3 : 2;        // waves per SIMD that the registers are held to
 };
 
 constexpr float kv8_head = 6.f, kv8_move = 14.f;       // the reference lies 2^6 under its maximum and moves above 2^14
 
-template <int HD, int NT, bool F16, int OT>
-__global__ void __launch_bounds__(256, (Kv8DecCfg<HD, NT>::OCC)) kv8_decode_kernel(const Kv8DecArgs a) {
+// STREAM: no other workgroup reads these keys; non-temporal loads sustain a higher HBM rate.
+template <int HD, int NT, bool F16, bool STREAM>
+__global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, NT>::OCC)) kv8_decode_kernel(const Kv8DecArgs a) {
     using Cf = Kv8DecCfg<HD, NT>;
-    constexpr int NW = Cf::NW, DC = Cf::DC, DB = Cf::DB;
+    constexpr int NW = Cf::NW, KT = Cf::KT, DC = Cf::DC, DB = Cf::DB, SK = Cf::SK;
     extern __shared__ __align__(16) unsigned char smem[];
     const Kv8Problem &p = a.p;
     const Kv8 &kc = p.c;
@@ -101,89 +106,105 @@ __global__ void __launch_bounds__(256, (Kv8DecCfg<HD, NT>::OCC)) kv8_decode_kern
     const int h = unit % kc.NKV, G = p.NQ / kc.NKV;
     int row0, nr;
     kv8_rows(p, seq, row0, nr);
+    row0 = __builtin_amdgcn_readfirstlane(row0); nr = __builtin_amdgcn_readfirstlane(nr);
     const int rho0 = rg * Cf::RR, nrows = min(nr * G - rho0, Cf::RR);
     const int j_lo = max(c * a.C, lo), j_hi = min(hi - c * a.C, a.C) + c * a.C;
     if (nrows <= 0 || (j_lo >= j_hi && !a.direct)) return;
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, ln = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int p0 = p.ctx[seq], page = kc.page;
+    const int p0 = scalar_load(p.ctx + seq), page = kc.page;
     const int *tab = p.table + (size_t)seq * p.table_stride;
     const int last_col = p.max_pos >> kc.lp;
+    auto safe = [&](int id) { return (unsigned)id < (unsigned)kc.pages ? id : 0; };
 
-    // The pages of a step: of the lane's K rows (16-key piece ln / 4), and of its scores and V columns (piece g).
-    struct Pages { int k, v; };
-    auto pages_of = [&](int s) {
-        Pages q;
-        q.k = tab[min((64 * s + 16 * (ln >> 2)) >> kc.lp, last_col)];
-        q.v = tab[min((64 * s + 16 * g) >> kc.lp, last_col)];
+    // Pages of a step's eight 16-key pieces, and the scales of the wave's own KT: uniform, loaded a step or two ahead.
+    struct Ids { int p[8]; };
+    auto ids_of = [&](int s) {
+        Ids q;
+#pragma unroll
+        for (int i = 0; i < 8; i++) q.p[i] = scalar_load(tab + min((SK * s + 16 * i) >> kc.lp, last_col));
         return q;
     };
-    u32x4 kr[4][DC], vr[DB];
-    float ksc, vsc;
-    bool vok;
-    auto safe = [&](int id) { return (unsigned)id < (unsigned)kc.pages ? id : 0; };
-    auto load_k = [&](int s, const Pages &q) {
-        const int key = 64 * s + 16 * (ln >> 2) + (ln & 3);
-        const uint8_t *b = kc.K + (((size_t)safe(q.k) * kc.NKV + h) * page + (key & (page - 1))) * HD + 16 * g;
+    struct Scales { float k[KT], v[KT]; bool ok[KT], all; };
+    auto scales_of = [&](const Ids &q) {
+        Scales r;
+        r.all = true;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int i = 0; i < 8; i++) r.all &= (unsigned)q.p[i] < (unsigned)kc.pages;
 #pragma unroll
-            for (int d = 0; d < DC; d++) kr[t][d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(b + 4 * t * HD + 64 * d));
+        for (int t = 0; t < KT; t++) {
+            int id = q.p[t];
+#pragma unroll
+            for (int w = 1; w < NW; w++) id = wave == w ? q.p[KT * w + t] : id;
+            const size_t cell = (size_t)safe(id) * kc.NKV + h;
+            r.ok[t] = (unsigned)id < (unsigned)kc.pages;
+            r.k[t] = scalar_load(kc.Ks + cell); r.v[t] = scalar_load(kc.Vs + cell);
+        }
+        return r;
     };
-    auto load_v = [&](int s, const Pages &q) {
-        const size_t cell = (size_t)safe(q.v) * kc.NKV + h;
-        const uint8_t *b = kc.V + (cell * HD + ln) * page + ((64 * s + 16 * g) & (page - 1));
-        ksc = kc.Ks[cell]; vsc = kc.Vs[cell];
-        vok = (unsigned)q.v < (unsigned)kc.pages;
+    const size_t head_bytes = (size_t)page * HD;
+    auto fetch = [](const uint8_t *q) {
+        if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(q));
+        else return *reinterpret_cast<const u32x4 *>(q);
+    };
+    u32x4 kr[KT][DC], vr[2][DB];
+    const unsigned klane = (unsigned)(ln * HD + 16 * g);
+    auto load_k = [&](int s, const Ids &q) {                           // tile t: key 16 (KT wave + t) + ln of the step
 #pragma unroll
-        for (int d = 0; d < DB; d++) vr[d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(b + (size_t)16 * d * page));
+        for (int t = 0; t < KT; t++) {
+            int id = q.p[t];
+#pragma unroll
+            for (int w = 1; w < NW; w++) id = wave == w ? q.p[KT * w + t] : id;
+            const uint8_t *b = kc.K + ((size_t)safe(id) * kc.NKV + h) * head_bytes + (size_t)((SK * s + 16 * (KT * wave + t)) & (page - 1)) * HD;
+#pragma unroll
+            for (int d = 0; d < DC; d++) kr[t][d] = fetch(b + (klane + 64 * d));
+        }
+    };
+    const unsigned vlane = (unsigned)((wave * (HD / NW) + ln) * page);
+    auto load_v = [&](int s, const Ids &q) {                           // dims of the wave, 16 tokens from 64 k + 16 g of the step
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int id = g < 2 ? (g ? safe(q.p[4 * k + 1]) : safe(q.p[4 * k])) : g == 2 ? safe(q.p[4 * k + 2]) : safe(q.p[4 * k + 3]);
+            const uint8_t *b = kc.V + (size_t)(unsigned)(id * kc.NKV + h) * head_bytes + (vlane + ((16 * g) & (page - 1)));
+#pragma unroll
+            for (int d = 0; d < DB; d++) vr[k][d] = fetch(b + 16 * d * page);
+        }
+        (void)s;
     };
 
-    // Wave w takes the steps w, w + NW, .. of the chunk's.
-    const int sc = c * (a.C / 64), s1 = j_hi > j_lo ? (j_hi - 1) / 64 : -1;
-    int s = j_lo / 64;
-    s += (wave - (s - sc)) & (NW - 1);
-    Pages pg{0, 0}, pn{0, 0};
+    const int s1 = j_hi > j_lo ? (j_hi - 1) / SK : -1;
+    int s = j_lo / SK;
+    Ids nxt{};
+    Scales sn{};
     if (s <= s1) {
-        pg = pages_of(s);
-        pn = pages_of(min(s + NW, s1));
+        const Ids q = ids_of(s);
+        nxt = ids_of(min(s + 1, s1));
+        load_k(s, q);
+        load_v(s, q);
+        sn = scales_of(q);
     }
     // Q rows, zeros past the last.
-    uint16_t *qs = reinterpret_cast<uint16_t *>(smem);
-    {
-        constexpr int N = Cf::RR * (HD / 8) / (NW * 64);
-        u32x4 v[N];
-#pragma unroll
-        for (int u = 0; u < N; u++) {
-            const int i = tid + NW * 64 * u, R = i / (HD / 8), rho = rho0 + R;
-            v[u] = u32x4{0u, 0u, 0u, 0u};
-            if (R < nrows)
-                v[u] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(p.Q) +
-                                                        ((size_t)(row0 + rho / G) * p.NQ + h * G + rho % G) * HD + (i % (HD / 8)) * 8);
-        }
-        if (s <= s1) { load_k(s, pg); load_v(s, pg); }
-#pragma unroll
-        for (int u = 0; u < N; u++) {
-            const int i = tid + NW * 64 * u;
-            *reinterpret_cast<u32x4 *>(qs + (i / (HD / 8)) * Cf::QSTR + (i % (HD / 8)) * 8) = v[u];
-        }
+    uint16_t *qs = reinterpret_cast<uint16_t *>(smem), *ps = reinterpret_cast<uint16_t *>(smem + Cf::LDS_Q);
+    float *red = reinterpret_cast<float *>(smem + Cf::LDS_Q + Cf::LDS_P);
+    for (int i = tid; i < Cf::RR * (HD / 8); i += NW * 64) {
+        const int R = i / (HD / 8), rho = rho0 + R;
+        u32x4 v{0u, 0u, 0u, 0u};
+        if (R < nrows)
+            v = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(p.Q) + ((size_t)(row0 + rho / G) * p.NQ + h * G + rho % G) * HD + (i % (HD / 8)) * 8);
+        *reinterpret_cast<u32x4 *>(qs + R * Cf::QSTR + (i % (HD / 8)) * 8) = v;
     }
-    RowMask rm[NT];
-    int lo_max = 0, pos_min = INT_MAX;
-    {
-        const int t0 = rho0 / G, t1 = (rho0 + nrows - 1) / G;
-        lo_max = win_lo(p0 + t1, p.window);
-        pos_min = p.anc ? p0 - 1 : p0 + t0;                            // tree keys: per row
+    // Rows of the lane (16 nt + ln) and the bounds within which no row needs its mask.
+    int rpos[NT];
+    uint32_t ranc[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int rho = rho0 + 16 * nt + ln;
-            rm[nt].valid = 16 * nt + ln < nrows;
-            const int t = rm[nt].valid ? rho / G : 0;
-            rm[nt].pos = p0 + t; rm[nt].lo = win_lo(p0 + t, p.window); rm[nt].tb = p0; rm[nt].tree = p.anc != nullptr;
-            rm[nt].anc = p.anc ? p.anc[row0 + t] : 0u;
-        }
+    for (int nt = 0; nt < NT; nt++) {
+        const int R = 16 * nt + ln, t = R < nrows ? (rho0 + R) / G : 0;
+        rpos[nt] = R < nrows ? p0 + t : -1;
+        ranc[nt] = p.anc && R < nrows ? p.anc[row0 + t] : 0u;
     }
+    const int t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
+    const int lo_max = win_lo(p0 + t_b, p.window), pos_min = p.anc ? p0 - 1 : p0 + t_a;
     __syncthreads();
 
     float m[NT], l[NT];
@@ -194,52 +215,70 @@ __global__ void __launch_bounds__(256, (Kv8DecCfg<HD, NT>::OCC)) kv8_decode_kern
 #pragma unroll
         for (int d = 0; d < DB; d++) acc[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (; s <= s1; s += NW) {
-        const int j0 = 64 * s;
-        const bool more = s + NW <= s1;
-        f32x4 st[4][NT];
+    for (; s <= s1; s++) {
+        const int j0 = SK * s, jw = j0 + 16 * KT * wave;
+        const Scales sc = sn;
+        f32x4 st[KT][NT];
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) st[t][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        unsigned qo = (unsigned)(ln * Cf::QSTR + 16 * g);              // (opaque: the fragments are read here, not held across steps)
+        asm volatile("" : "+v"(qo));
 #pragma unroll
         for (int d = 0; d < DC; d++) {
-            u32x4 q[NT][2];
+            u32x4 k0[KT], k1[KT];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int t = 0; t < KT; t++) { k0[t] = e4m3_op<F16>(kr[t][d][0], kr[t][d][1]); k1[t] = e4m3_op<F16>(kr[t][d][2], kr[t][d][3]); }
 #pragma unroll
-                for (int e = 0; e < 2; e++) q[nt][e] = *reinterpret_cast<const u32x4 *>(qs + (16 * nt + ln) * Cf::QSTR + 64 * d + 16 * g + 8 * e);
+            for (int nt = 0; nt < NT; nt++) {
+                const u32x4 q0 = *reinterpret_cast<const u32x4 *>(qs + qo + 16 * nt * Cf::QSTR + 64 * d);
+                const u32x4 q1 = *reinterpret_cast<const u32x4 *>(qs + qo + 16 * nt * Cf::QSTR + 64 * d + 8);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const u32x4 k0 = e4m3_op<F16>(kr[t][d][0], kr[t][d][1]), k1 = e4m3_op<F16>(kr[t][d][2], kr[t][d][3]);
+                for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k0[t], q0, st[t][nt]);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) st[t][nt] = mfma16<F16>(k0, q[nt][0], st[t][nt]);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) st[t][nt] = mfma16<F16>(k1, q[nt][1], st[t][nt]);
+                for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k1[t], q1, st[t][nt]);
             }
         }
-        const float kf = ksc * a.sl2, ev = (float)exp_of(vsc), iv = pow2i(-exp_of(vsc));
-        const bool ok = vok;
-        if (more) load_k(s + NW, pn);
-        const bool part = j0 < j_lo || j0 + 64 > j_hi || __any(!ok);   // keys of the step outside the chunk's, or without a page
-        const bool full = !part && j0 >= lo_max && j0 + 63 <= pos_min;
-        u32x2 pf[NT][4];                                               // P of tile t: the lane's keys 16 g + 4 t ..
+        Ids cur = nxt;
+        if (s < s1) {
+            load_k(s + 1, cur);
+            sn = scales_of(cur);
+            nxt = ids_of(min(s + 2, s1));
+        }
+        bool pages_ok = true;
+#pragma unroll
+        for (int t = 0; t < KT; t++) pages_ok &= sc.ok[t];
+        const bool full = pages_ok && jw >= j_lo && jw + 16 * KT <= j_hi && jw >= lo_max && jw + 16 * KT - 1 <= pos_min;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float tv[16];
+            float mx = kNegInf;
 #pragma unroll
-            for (int i = 0; i < 16; i++) tv[i] = __builtin_fmaf(st[i >> 2][nt][i & 3], kf, ev);
-            if (!full) {
+            for (int t = 0; t < KT; t++) {
+                const float kf = sc.k[t] * a.sl2, ev = (float)exp_of(sc.v[t]);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int key = j0 + 16 * g + i;
-                    if (!(ok & (key >= j_lo) & (key < j_hi) & rm[nt].attends(key))) tv[i] = kNegInf;
+                for (int i = 0; i < 4; i++) st[t][nt][i] = __builtin_fmaf(st[t][nt][i], kf, ev);
+                if (!full) {
+                    const int kb = jw + 16 * t + 4 * g, kl = max(j_lo, win_lo(rpos[nt], p.window)) - kb, kh = sc.ok[t] ? min(j_hi - 1, rpos[nt]) - kb : -1;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        bool out = (i < kl) | (i > kh);
+                        if (p.anc) { const int d = kb + i - p0; out |= (d >= 0) & ((d >= 32) | !((ranc[nt] >> (d & 31)) & 1u)); }
+                        if (out) st[t][nt][i] = kNegInf;
+                    }
                 }
-            }
-            float mx = tv[0];
 #pragma unroll
-            for (int i = 1; i < 16; i++) mx = fmaxf(mx, tv[i]);
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[t][nt][i]);
+            }
             mx = max_over_groups(mx);
+            if (g == 0) red[wave * Cf::RR + 16 * nt + ln] = mx;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float mx = red[16 * nt + ln];
+#pragma unroll
+            for (int w = 1; w < NW; w++) mx = fmaxf(mx, red[w * Cf::RR + 16 * nt + ln]);
             const float mn = mx > m[nt] + kv8_move ? mx - kv8_head : m[nt];
             if (__any(mn != m[nt])) {
                 const float al = mn == m[nt] ? 1.f : fast_exp2(m[nt] - mn);
@@ -247,98 +286,84 @@ __global__ void __launch_bounds__(256, (Kv8DecCfg<HD, NT>::OCC)) kv8_decode_kern
 #pragma unroll
                 for (int d = 0; d < DB; d++) acc[nt][d] *= al;
             }
-            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                if (full) tv[i] = fast_exp2(tv[i] - m[nt]);
-                else tv[i] = tv[i] == kNegInf ? 0.f : fast_exp2(tv[i] - m[nt]);        // (a row without a key yet: m = -inf)
-                sum += tv[i];
+            for (int t = 0; t < KT; t++) {
+                float pv[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = st[t][nt][i];
+                    pv[i] = full ? fast_exp2(x - m[nt]) : x == kNegInf ? 0.f : fast_exp2(x - m[nt]);   // (a row without a key yet: m = -inf)
+                }
+                l[nt] = __builtin_fmaf((pv[0] + pv[1]) + (pv[2] + pv[3]), pow2i(-exp_of(sc.v[t])), l[nt]);
+                *reinterpret_cast<u32x2 *>(ps + (16 * nt + ln) * Cf::PSTR + 16 * (KT * wave + t) + 4 * g) =
+                    u32x2{pack2<true>(pv[0], pv[1]), pack2<true>(pv[2], pv[3])};
             }
-            l[nt] = __builtin_fmaf(sum, iv, l[nt]);
-#pragma unroll
-            for (int t = 0; t < 4; t++) pf[nt][t] = u32x2{pack2<true>(tv[4 * t], tv[4 * t + 1]), pack2<true>(tv[4 * t + 2], tv[4 * t + 3])};
         }
-        if (part) {                                                    // bytes that are no token of the request's: any code, NaN too
-            const int k0 = ok ? max(j_lo - j0 - 16 * g, 0) : 16, k1 = min(j_hi - j0 - 16 * g, 16);
-            u32x4 keep;
+        __syncthreads();
+        if (!sc.all || j0 < j_lo || j0 + SK > j_hi) {                  // bytes that are no token of the request's: any code, NaN too
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const int x = min(max(k0 - 4 * w, 0), 4), y = min(max(k1 - 4 * w, 0), 4);      // bytes [x, y) of word w
-                const uint32_t below = y >= 4 ? 0xffffffffu : (1u << (8 * y)) - 1u, under = x >= 4 ? 0xffffffffu : (1u << (8 * x)) - 1u;
-                keep[w] = below & ~under;
+            for (int k = 0; k < 2; k++) {
+                // (a page outside the pool was read as page 0, whose codes may be NaN: its id is gone here, the table is read again)
+                const int jb = j0 + 64 * k + 16 * g, id = tab[min(jb >> kc.lp, last_col)];
+                const int k0 = (unsigned)id < (unsigned)kc.pages ? max(j_lo - jb, 0) : 16, k1 = min(j_hi - jb, 16);
+                u32x4 keep;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int x = min(max(k0 - 4 * w, 0), 4), y = min(max(k1 - 4 * w, 0), 4);      // bytes [x, y) of word w
+                    keep[w] = (y >= 4 ? 0xffffffffu : (1u << (8 * y)) - 1u) & ~(x >= 4 ? 0xffffffffu : (1u << (8 * x)) - 1u);
+                }
+#pragma unroll
+                for (int d = 0; d < DB; d++) vr[k][d] &= keep;
             }
-#pragma unroll
-            for (int d = 0; d < DB; d++) vr[d] &= keep;
         }
-        if (more) pg = pn;
+        unsigned po = (unsigned)(ln * Cf::PSTR + 16 * g);
+        asm volatile("" : "+v"(po));
 #pragma unroll
-        for (int d = 0; d < DB; d++) {
-            const u32x4 v0 = e4m3_op<true>(vr[d][0], vr[d][1]), v1 = e4m3_op<true>(vr[d][2], vr[d][3]);
+        for (int k = 0; k < 2; k++) {
+            u32x4 pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
-                acc[nt][d] = mfma16<true>(v0, u32x4{pf[nt][0][0], pf[nt][0][1], pf[nt][1][0], pf[nt][1][1]}, acc[nt][d]);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                acc[nt][d] = mfma16<true>(v1, u32x4{pf[nt][2][0], pf[nt][2][1], pf[nt][3][0], pf[nt][3][1]}, acc[nt][d]);
+                for (int e = 0; e < 2; e++) pf[nt][e] = *reinterpret_cast<const u32x4 *>(ps + po + 16 * nt * Cf::PSTR + 64 * k + 8 * e);
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const u32x4 v0 = e4m3_op<true>(vr[k][d][0], vr[k][d][1]), v1 = e4m3_op<true>(vr[k][d][2], vr[k][d][3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) acc[nt][d] = mfma16<true>(v0, pf[nt][0], acc[nt][d]);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) acc[nt][d] = mfma16<true>(v1, pf[nt][1], acc[nt][d]);
+            }
         }
-        if (more) {
-            load_v(s + NW, pg);
-            pn = pages_of(min(s + 2 * NW, s1));
-        }
+        if (s < s1) load_v(s + 1, cur);
     }
 
-    // Merge the waves' states in their order.
-    float *redm = reinterpret_cast<float *>(smem), *redl = redm + NW * Cf::RR, *buf = redl + NW * Cf::RR;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) l[nt] = sum_over_groups(l[nt]);
+    // Row sums over the waves, in their order; m is the same in all.
     __syncthreads();
-    if (g == 0)
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) { redm[wave * Cf::RR + 16 * nt + ln] = m[nt]; redl[wave * Cf::RR + 16 * nt + ln] = l[nt]; }
-    __syncthreads();
-    for (int w = 0; w < NW; w++) {
-        if (wave == w)
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (16 * nt + ln >= nrows) continue;
-                float M = kNegInf;
-#pragma unroll
-                for (int x = 0; x < NW; x++) M = fmaxf(M, redm[x * Cf::RR + 16 * nt + ln]);
-                const float f = kv8_weight(m[nt], l[nt], M);
-#pragma unroll
-                for (int d = 0; d < DB; d++) {
-                    f32x4 *dst = reinterpret_cast<f32x4 *>(buf + (16 * nt + ln) * Cf::BSTR + 16 * d + 4 * g);
-                    f32x4 v = acc[nt][d] * f;
-                    if (w > 0) v += *dst;
-                    *dst = v;
-                }
-            }
-        __syncthreads();
+    for (int nt = 0; nt < NT; nt++) {
+        l[nt] = sum_over_groups(l[nt]);
+        if (g == 0) red[wave * Cf::RR + 16 * nt + ln] = l[nt];
     }
-    auto state_of = [&](int R, float &M, float &L) {
-        M = kNegInf; L = 0.f;
-        for (int x = 0; x < NW; x++) M = fmaxf(M, redm[x * Cf::RR + R]);
-        for (int x = 0; x < NW; x++) {
-            const float mx = redm[x * Cf::RR + R], lx = redl[x * Cf::RR + R];
-            L += mx == kNegInf ? lx * 0.f : lx * fast_exp2(mx - M);
-        }
-    };
-    for (int i = tid; i < nrows * (HD / 4); i += NW * 64) {
-        const int R = i / (HD / 4), d4 = i % (HD / 4), rho = rho0 + R;
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int R = 16 * nt + ln, rho = rho0 + R;
+        if (R >= nrows) continue;
+        float L = red[R];
+#pragma unroll
+        for (int w = 1; w < NW; w++) L += red[w * Cf::RR + R];
         const size_t row = (size_t)(row0 + rho / G) * p.NQ + h * G + rho % G;
-        f32x4 v = *reinterpret_cast<const f32x4 *>(buf + R * Cf::BSTR + 4 * d4);
-        float M, L;
-        state_of(R, M, L);
+        const int dim0 = wave * (HD / NW) + 4 * g;
         if (a.direct) {
-            v *= L == 0.f ? 0.f : 1.f / L;
-            if constexpr (OT == DT_FP32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.O) + row * HD + 4 * d4) = v;
-            else *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.O) + row * HD + 4 * d4) =
-                u32x2{pack2<OT == DT_F16>(v[0], v[1]), pack2<OT == DT_F16>(v[2], v[3])};
-            if (d4 == 0 && p.lse) p.lse[row] = L == 0.f ? kNegInf : (M + __builtin_amdgcn_logf(L)) * kLn2;
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+            for (int d = 0; d < DB; d++) kv8_store4(p, row * HD + dim0 + 16 * d, acc[nt][d] * inv);
+            if (wave == 0 && g == 0 && p.lse) p.lse[row] = L == 0.f ? kNegInf : (m[nt] + __builtin_amdgcn_logf(L)) * kLn2;
         } else {
             const size_t x = row * a.part.ns + c;
-            *reinterpret_cast<f32x4 *>(a.part.acc + x * HD + 4 * d4) = v;
-            if (d4 == 0) { a.part.m[x] = M; a.part.l[x] = L; }
+#pragma unroll
+            for (int d = 0; d < DB; d++) *reinterpret_cast<f32x4 *>(a.part.acc + x * HD + dim0 + 16 * d) = acc[nt][d];
+            if (wave == 0 && g == 0) { a.part.m[x] = m[nt]; a.part.l[x] = L; }
         }
     }
 }
@@ -352,7 +377,7 @@ struct Kv8CombArgs {
     uint32_t Cm;
 };
 
-template <int HD, int OT>
+template <int HD>
 __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8CombArgs a) {
     constexpr int TPR = HD / 4, PH = 256 / TPR;
     __shared__ __align__(16) float red[PH][HD];
@@ -381,18 +406,12 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8CombArgs a) {
         for (int x = 1; x < PH; x++) v += *reinterpret_cast<const f32x4 *>(&red[x][4 * d4]);
     }
     v *= L == 0.f ? 0.f : 1.f / L;
-    if constexpr (OT == DT_FP32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.O) + row * HD + 4 * d4) = v;
-    else *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.O) + row * HD + 4 * d4) =
-        u32x2{pack2<OT == DT_F16>(v[0], v[1]), pack2<OT == DT_F16>(v[2], v[3])};
+    kv8_store4(p, row * HD + 4 * d4, v);
     if (d4 == 0 && p.lse) p.lse[row] = L == 0.f ? kNegInf : (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
 template <int HD> static hipError_t combine_t(const Kv8CombArgs &a, dim3 grid, hipStream_t st) {
-    switch (a.p.o_dtype) {
-    case DT_FP32: hipLaunchKernelGGL((kv8_combine_kernel<HD, DT_FP32>), grid, dim3(256), 0, st, a); break;
-    case DT_F16: hipLaunchKernelGGL((kv8_combine_kernel<HD, DT_F16>), grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL((kv8_combine_kernel<HD, DT_BF16>), grid, dim3(256), 0, st, a); break;
-    }
+    hipLaunchKernelGGL(kv8_combine_kernel<HD>, grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -408,27 +427,17 @@ hipError_t launch_kv8_combine(const Kv8Problem &p, const Kv8Partials &part, hipS
 }
 
 // ---------------------------------------------------------------- launch
-template <int HD, int NT, bool F16, int OT>
+template <int HD, int NT, bool F16, bool STREAM>
 static hipError_t launch_dec_k(const Kv8DecArgs &a, dim3 grid, hipStream_t st) {
     using Cf = Kv8DecCfg<HD, NT>;
-    static_assert(Cf::LDS <= 160 * 1024, "LDS");
-    if constexpr (Cf::LDS > 64 * 1024) {                               // per device; setting it again changes nothing
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv8_decode_kernel<HD, NT, F16, OT>),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)Cf::LDS);
-        if (e != hipSuccess) return e;
-    }
-    hipLaunchKernelGGL((kv8_decode_kernel<HD, NT, F16, OT>), grid, dim3(Cf::NW * 64), Cf::LDS, st, a);
+    static_assert(Cf::LDS <= 64 * 1024, "LDS");
+    hipLaunchKernelGGL((kv8_decode_kernel<HD, NT, F16, STREAM>), grid, dim3(Cf::NW * 64), Cf::LDS, st, a);
     return hipGetLastError();
 }
-template <int HD, int NT, bool F16> static hipError_t launch_dec_o(const Kv8DecArgs &a, dim3 grid, hipStream_t st) {
-    switch (a.p.o_dtype) {
-    case DT_FP32: return launch_dec_k<HD, NT, F16, DT_FP32>(a, grid, st);
-    case DT_F16: return launch_dec_k<HD, NT, F16, DT_F16>(a, grid, st);
-    default: return launch_dec_k<HD, NT, F16, DT_BF16>(a, grid, st);
-    }
-}
 template <int HD, int NT> static hipError_t launch_dec_n(const Kv8DecArgs &a, dim3 grid, hipStream_t st) {
-    return a.p.q_dtype == DT_F16 ? launch_dec_o<HD, NT, true>(a, grid, st) : launch_dec_o<HD, NT, false>(a, grid, st);
+    const bool f16 = a.p.q_dtype == DT_F16;
+    if (a.nrg == 1) return f16 ? launch_dec_k<HD, NT, true, true>(a, grid, st) : launch_dec_k<HD, NT, false, true>(a, grid, st);
+    return f16 ? launch_dec_k<HD, NT, true, false>(a, grid, st) : launch_dec_k<HD, NT, false, false>(a, grid, st);
 }
 
 Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, bool tree) {
@@ -450,7 +459,7 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
 
 hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st) {
     const int G = p.NQ / p.c.NKV, rows = (int)std::min<long long>((long long)p.T * G, INT_MAX);
-    const int nt = p.c.HD == 512 || rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int nt = rows <= 16 ? 1 : rows <= 32 || p.c.HD == 512 ? 2 : 4;
     Kv8DecArgs a{p, part, part.C, div_magic(part.C), (rows + 16 * nt - 1) / (16 * nt), part.ns == 1, p.scale * kLog2e};
     long long per = p.max_pos / part.C + 1;
     if (p.window > 0) per = std::min<long long>(per, ((long long)p.window + p.T - 2) / part.C + 2);
@@ -460,7 +469,7 @@ hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, hipSt
     switch (p.c.HD) {
     case 128: return nt == 1 ? launch_dec_n<128, 1>(a, grid, st) : nt == 2 ? launch_dec_n<128, 2>(a, grid, st) : launch_dec_n<128, 4>(a, grid, st);
     case 256: return nt == 1 ? launch_dec_n<256, 1>(a, grid, st) : nt == 2 ? launch_dec_n<256, 2>(a, grid, st) : launch_dec_n<256, 4>(a, grid, st);
-    case 512: return launch_dec_n<512, 1>(a, grid, st);
+    case 512: return nt == 1 ? launch_dec_n<512, 1>(a, grid, st) : launch_dec_n<512, 2>(a, grid, st);
     default: return hipErrorInvalidValue;
     }
 }
