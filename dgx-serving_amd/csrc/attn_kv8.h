@@ -42,11 +42,10 @@ template <bool F16, bool HI> __device__ __forceinline__ uint32_t e4m3_pair(uint3
 template <bool F16> __device__ __forceinline__ u32x4 e4m3_op(uint32_t w0, uint32_t w1) {
     return u32x4{e4m3_pair<F16, false>(w0), e4m3_pair<F16, true>(w0), e4m3_pair<F16, false>(w1), e4m3_pair<F16, true>(w1)};
 }
-// Four finite values to e4m3 codes: nearest, ties to even; values past +-448 (possible only at kv8_emax) become +-448.
+// Four values of at most 448 to e4m3 codes: nearest, ties to even.
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
-    auto lim = [](float x) { return __builtin_amdgcn_fmed3f(x, -448.f, 448.f); };
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(lim(a), lim(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lim(c), lim(d), w, true);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
 // One call of the attention: row r of Q / O / lse belongs to request b for r in [cu[b], cu[b + 1]) (cu null: T rows each),

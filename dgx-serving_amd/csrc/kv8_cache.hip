@@ -13,10 +13,10 @@ namespace dgx {
 // All or nothing: a step that needs more free pages, columns or rows than there are, or has a negative length, takes nothing
 // (status tells which), gives every row slot -1 and every request no rows.
 //
-// The scans take one workgroup's time whatever the grid, so every workgroup does them (lengths come from the L2) and takes
-// its share of the rows; a second launch behind a one-workgroup scan would cost more than the scan. One workgroup alone
-// does it all where the free count is updated in place (another workgroup could read it late), or for up to 8192 rows: 256
-// requests of one token 5.4 us a call either way.
+// Bound by latency: lengths, scan, free ids, slots. The scans take one workgroup's time whatever the grid, so every workgroup
+// does them (lengths come from the L2) and takes its share of the rows; a second launch behind a one-workgroup scan would
+// cost more than the scan. One workgroup alone does it all where the free count is updated in place (another workgroup
+// could read it late), and for up to 8192 rows.
 struct PlanArgs {
     const int *ctx, *add, *free_pages, *free_in;
     int *table, *free_out, *cu, *slots, *status;
@@ -26,7 +26,11 @@ struct PlanArgs {
 
 constexpr int kPlanThreads = 1024;
 
-__device__ __forceinline__ long long scan64(long long v) {        // inclusive, over the wave
+// Lengths are clamped to what a step can hold (and the step is refused): with at most kNarrow rows and columns the sums of
+// 1024 requests fit 32 bits, whose scans are a fifth of the work.
+constexpr int kNarrow = 1 << 20;
+__device__ __forceinline__ int scan_wave(int v) { return wave_scan64(v); }
+__device__ __forceinline__ long long scan_wave(long long v) {     // inclusive
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -36,43 +40,51 @@ __device__ __forceinline__ long long scan64(long long v) {        // inclusive, 
     return v;
 }
 
+template <class T>
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a) {
-    __shared__ long long w_pages[kPlanThreads / 64], w_rows[kPlanThreads / 64];
+    __shared__ T w_pages[kPlanThreads / 64], w_rows[kPlanThreads / 64];
     __shared__ int s_row[kPlanThreads + 1], s_page[kPlanThreads], s_ctx[kPlanThreads], bad_s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, page = 1 << a.lp;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, page = 1 << a.lp;
     const int count = a.free_in[0];
-    if (tid == 0) bad_s = (count < 0 || count > a.free_cap) ? 8 : 0;
-    __syncthreads();
-    // Lengths of request b, pages and rows that it takes; 64 bits where sums of the callers' numbers could pass 32.
-    auto lengths = [&](int b, int &ctx, long long &pages, long long &rows, int &flags) {
+    int flags = count < 0 || count > a.free_cap ? 8 : 0;
+    // Lengths of request b: pages and rows that it takes.
+    auto lengths = [&](int b, int &ctx, T &pages, T &rows) {
         ctx = 0; pages = rows = 0;
         if (b >= a.B) return;
         const int c = a.ctx[b], n = a.add[b];
-        if (c < 0 || n < 0) { flags |= 8; return; }
         const long long have = ((long long)c + page - 1) >> a.lp, want = ((long long)c + n + page - 1) >> a.lp;
-        if (want > a.cols) flags |= 2;
-        ctx = c; pages = want - have; rows = n;
+        const int f = (c < 0 || n < 0 ? 8 : 0) | (want > a.cols ? 2 : 0) | (n > a.rows ? 4 : 0);
+        flags |= f;
+        if (f) return;
+        ctx = c; pages = (T)(want - have); rows = n;
     };
-    // Workgroup-wide inclusive scans of pages and rows.
-    auto scan = [&](long long &pages, long long &rows, long long &all_pages, long long &all_rows) {
-        pages = scan64(pages); rows = scan64(rows);
-        __syncthreads();
+    // Workgroup-wide inclusive scans of pages and rows, and the totals.
+    auto scan = [&](T &pages, T &rows, T &all_pages, T &all_rows) {
+        pages = scan_wave(pages); rows = scan_wave(rows);
         if (lane == 63) { w_pages[wave] = pages; w_rows[wave] = rows; }
         __syncthreads();
         all_pages = all_rows = 0;
-        for (int w = 0; w < kPlanThreads / 64; w++) {
-            if (w == wave) { pages += all_pages; rows += all_rows; }
+        T before_p = 0, before_r = 0;
+        for (int w = 0; w < nt / 64; w++) {
+            if (w == wave) { before_p = all_pages; before_r = all_rows; }
             all_pages += w_pages[w]; all_rows += w_rows[w];
         }
+        pages += before_p; rows += before_r;
     };
-    long long need_pages = 0, need_rows = 0;                       // totals over all requests
-    int flags = 0;
-    for (int t0 = 0; t0 < a.B; t0 += kPlanThreads) {
-        int ctx;
-        long long pages, rows, ap, ar;
-        lengths(t0 + tid, ctx, pages, rows, flags);
-        scan(pages, rows, ap, ar);
-        need_pages += ap; need_rows += ar;
+    if (tid == 0) bad_s = 0;
+    int ctx;
+    T pages, rows, ap, ar;
+    lengths(tid, ctx, pages, rows);
+    T mine = pages;
+    scan(pages, rows, ap, ar);                                     // (its barrier is behind bad_s = 0 too)
+    long long need_pages = ap, need_rows = ar;
+    for (int t0 = nt; t0 < a.B; t0 += nt) {                        // totals over the requests behind the first tile
+        int c;
+        T x, y, xp, yr;
+        lengths(t0 + tid, c, x, y);
+        __syncthreads();
+        scan(x, y, xp, yr);
+        need_pages += xp; need_rows += yr;
     }
     if (need_pages > max(count, 0)) flags |= 1;
     if (need_rows > a.rows) flags |= 4;
@@ -88,26 +100,21 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
             a.cu[0] = 0;
         }
         if (bad)
-            for (int b = tid; b < a.B; b += kPlanThreads) a.cu[b + 1] = 0;
+            for (int b = tid; b < a.B; b += nt) a.cu[b + 1] = 0;
     }
-    for (long long r = max(r_lo, bad ? 0ll : need_rows) + tid; r < r_hi; r += kPlanThreads) a.slots[r] = -1;
+    for (long long r = max(r_lo, bad ? 0ll : need_rows) + tid; r < r_hi; r += nt) a.slots[r] = -1;
     if (bad) return;
     long long base_pages = 0, base_rows = 0;
-    for (int t0 = 0; t0 < a.B; t0 += kPlanThreads) {               // 1024 requests at a time
-        int ctx, dummy = 0;
-        long long pages, rows, ap, ar;
-        lengths(t0 + tid, ctx, pages, rows, dummy);
-        const long long own_pages = pages, own_rows = rows;
-        scan(pages, rows, ap, ar);
+    for (int t0 = 0;;) {                                           // a tile of requests at a time; the first one's scan is done
         s_row[tid + 1] = (int)(base_rows + rows);                  // (at most a.rows: checked above)
         if (tid == 0) s_row[0] = (int)base_rows;
-        s_page[tid] = (int)(base_pages + pages - own_pages);
+        s_page[tid] = (int)(base_pages + pages - mine);
         s_ctx[tid] = ctx;
         if (blockIdx.x == 0 && t0 + tid < a.B) a.cu[t0 + tid + 1] = (int)(base_rows + rows);
         __syncthreads();
-        const int nb = min(kPlanThreads, a.B - t0);
+        const int nb = min(nt, a.B - t0);
         const long long lo = max(r_lo, base_rows), hi = min(r_hi, base_rows + ar);
-        for (long long r = lo + tid; r < hi; r += kPlanThreads) {
+        for (long long r = lo + tid; r < hi; r += nt) {
             int x = 0, y = nb;                                     // the request: s_row[x] <= r < s_row[x + 1]
             while (y - x > 1) {
                 const int mid = (x + y) >> 1;
@@ -121,9 +128,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const PlanArgs a
             if (off == 0) *cell = id;
             a.slots[r] = id >= 0 && id <= (0x7fffffff >> a.lp) - 1 ? (id << a.lp) + off : -1;
         }
-        (void)own_rows;
         base_pages += ap; base_rows += ar;
+        t0 += nt;
+        if (t0 >= a.B) break;
         __syncthreads();
+        lengths(t0 + tid, ctx, pages, rows);
+        mine = pages;
+        scan(pages, rows, ap, ar);
     }
 }
 
@@ -132,7 +143,9 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
                            int *status, hipStream_t st) {
     const PlanArgs a{ctx, add, free_pages, free_in, table, free_out, cu, slots, status, table_stride, B, lp, cols, rows, free_cap};
     const int grid = free_in == free_out || rows <= 8192 ? 1 : std::min(128, (rows + 2047) / 2048);
-    hipLaunchKernelGGL(kv8_plan_kernel, dim3(grid), dim3(kPlanThreads), 0, st, a);
+    const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;     // fewer waves meet sooner at the barriers
+    if (rows <= kNarrow && cols <= kNarrow) hipLaunchKernelGGL(kv8_plan_kernel<int>, dim3(grid), dim3(threads), 0, st, a);
+    else hipLaunchKernelGGL(kv8_plan_kernel<long long>, dim3(grid), dim3(threads), 0, st, a);
     return hipGetLastError();
 }
 
@@ -155,7 +168,7 @@ struct AppendArgs {
     Kv8 c;
     const int *slots;
     unsigned *stats;                  // {non-finite K, V, max |K|, max |V|} or null
-    int rows, win, lv;                // rows of a workgroup's window; lv = log2(HD / 8)
+    int rows, win, lv, windows;       // win: rows of a workgroup's window; lv = log2(HD / 8)
 };
 
 // 8 values of a source row.
@@ -167,6 +180,13 @@ template <int ST> struct Src8 {
             const uint16_t h = (uint16_t)(w[0][i >> 1] >> (16 * (i & 1)));
             if constexpr (ST == DT_F16) return f16_bits_to_f32(h);
             else return bf16_bits_to_f32(h);
+        }
+    }
+    __device__ __forceinline__ void put(int i, float x) {              // x: a value of the type
+        if constexpr (ST == DT_FP32) w[i >> 2][i & 3] = __float_as_uint(x);
+        else {
+            const uint32_t h = f32_to_op(x, ST == DT_F16);
+            w[0][i >> 1] = (i & 1) ? (w[0][i >> 1] & 0xffffu) | (h << 16) : (w[0][i >> 1] & 0xffff0000u) | h;
         }
     }
 };
@@ -189,7 +209,11 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const AppendArgs a) {
     const Kv8 &c = a.c;
     const int page = c.page, HD = c.HD, PQ = page / 4;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, nw = (nt + 63) >> 6;
-    const int h = blockIdx.y, w0 = blockIdx.x * a.win;
+    // Workgroups go round-robin over the 8 XCDs and runs begin at regular distances: each XCD takes an eighth of the windows.
+    const unsigned unit = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int h = (int)(unit % (unsigned)c.NKV);
+    if (unit / (unsigned)c.NKV >= (unsigned)a.windows) return;
+    const int w0 = (int)(unit / (unsigned)c.NKV) * a.win;
     const int total = c.pages << c.lp;                             // host: at most INT_MAX
     unsigned long long starts;
     {
@@ -210,38 +234,54 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const AppendArgs a) {
         }
         for (int i = tid; i < 64; i += nt) bad_s[i] = 0;
         if (tid < 2) nonfin[tid] = 0;
+        // (Tokens behind the run repeat its last one: its magnitudes change nothing, and no load waits for a branch.)
         Src8<ST> x[2][4];
+        const bool live = 4 * tg < n;
+        if (live) {
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int tok = 4 * tg + i;
-                const SE *p = reinterpret_cast<const SE *>(t ? a.v : a.k) + (size_t)(r0 + tok) * (size_t)(t ? a.vs : a.ks) + h * HD + 8 * dv;
+                for (int i = 0; i < 4; i++) {
+                    const SE *p = reinterpret_cast<const SE *>(t ? a.v : a.k) + (size_t)(r0 + min(4 * tg + i, n - 1)) * (size_t)(t ? a.vs : a.ks) + h * HD + 8 * dv;
 #pragma unroll
-                for (int q = 0; q < (ST == DT_FP32 ? 2 : 1); q++)
-                    x[t][i].w[q] = tok < n ? __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p) + q) : u32x4{0u, 0u, 0u, 0u};
-            }
+                    for (int q = 0; q < (ST == DT_FP32 ? 2 : 1); q++) x[t][i].w[q] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p) + q);
+                }
+        }
         const size_t cell = (size_t)pid * c.NKV + h;
         const float oldk = c.Ks[cell], oldv = c.Vs[cell];
         __syncthreads();
-        float amax[2] = {0.f, 0.f};
+        constexpr uint32_t kInf = 0x7f800000u;
+        uint32_t top[2] = {0u, 0u};                                     // bits of the largest magnitude (they order as the values)
+        if (live) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top[t] = max(top[t], __float_as_uint(x[t][i].get(e)) & 0x7fffffffu);
+                if (top[t] >= kInf) {                                   // rare: something here is not finite
+                    top[t] = 0u;
+                    int nf = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const uint32_t m = __float_as_uint(x[t][i].get(e)) & 0x7fffffffu;
+                            if (m < kInf) top[t] = max(top[t], m);
+                            else {
+                                bad_s[4 * tg + i] = 1;
+                                nf += 4 * tg + i < n ? 1 : 0;
+                                x[t][i].put(e, 0.f);
+                            }
+                        }
+                    if (nf && a.stats) atomicAdd(&nonfin[t], nf);
+                }
+            }
+        }
+        float amax[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            int nf = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                int q = 0;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float m = fabsf(x[t][i].get(e));
-                    const bool fin = m < kPosInf;                   // (NaN compares false)
-                    amax[t] = fmaxf(amax[t], fin ? m : 0.f);
-                    q += fin ? 0 : 1;
-                }
-                if (q) bad_s[4 * tg + i] = 1;
-                nf += q;
-            }
-            if (nf && a.stats) atomicAdd(&nonfin[t], nf);
+            amax[t] = __uint_as_float(top[t]);
 #pragma unroll
             for (int d = 32; d; d >>= 1) amax[t] = fmaxf(amax[t], __shfl_xor(amax[t], d));
             if (lane == 0) red[t][tid >> 6] = amax[t];
@@ -294,35 +334,42 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const AppendArgs a) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         const float ik = pow2i(-e[0]), iv = pow2i(-e[1]);
-        uint32_t vc[4][2];
+        if (ST != DT_F16 && live && (e[0] == kv8_emax || e[1] == kv8_emax)) {   // the largest scale may be too small: values past 448 of it
+            const float top_v = 448.f * pow2i(kv8_emax);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int tok = 4 * tg + i;
-            const bool nan = bad_s[tok < 64 ? tok : 0] != 0;
-            float f[8];
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int q = 0; q < 8; q++) f[q] = x[0][i].get(q) * ik;
-            const u32x2 kc = nan ? u32x2{0x7f7f7f7fu, 0x7f7f7f7fu} : u32x2{to_e4m3x4(f[0], f[1], f[2], f[3]), to_e4m3x4(f[4], f[5], f[6], f[7])};
-            if (tok < n) *reinterpret_cast<u32x2 *>(Kp + (size_t)(off + tok) * HD + 8 * dv) = kc;
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                const float m = x[1][i].get(q);
-                f[q] = fabsf(m) < kPosInf ? m * iv : 0.f;
-            }
-            vc[i][0] = to_e4m3x4(f[0], f[1], f[2], f[3]);
-            vc[i][1] = to_e4m3x4(f[4], f[5], f[6], f[7]);
+                    for (int q = 0; q < 8; q++) x[t][i].put(q, __builtin_amdgcn_fmed3f(x[t][i].get(q), -top_v, top_v));
         }
-        // [4 tokens][8 dims] -> [8 dims][4 tokens]. Word (dim d, tokens 4 tq ..) of the tile sits at d * PQ + (tq ^ (d / 8 %
-        // PQ)): the lanes of a wave hold dims 8 apart, which would all share a bank.
         uint32_t *tw = reinterpret_cast<uint32_t *>(tile);
+        if (live) {
+            uint32_t vc[4][2];
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const uint32_t l01 = __builtin_amdgcn_perm(vc[1][q], vc[0][q], 0x05010400u), h01 = __builtin_amdgcn_perm(vc[1][q], vc[0][q], 0x07030602u);
-            const uint32_t l23 = __builtin_amdgcn_perm(vc[3][q], vc[2][q], 0x05010400u), h23 = __builtin_amdgcn_perm(vc[3][q], vc[2][q], 0x07030602u);
-            const uint32_t b[4] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
-                                   __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u)};
+            for (int i = 0; i < 4; i++) {
+                const int tok = 4 * tg + i;
+                const bool nan = bad_s[tok] != 0;
+                u32x2 kc;
 #pragma unroll
-            for (int d = 0; d < 4; d++) tw[(8 * dv + 4 * q + d) * PQ + (tg ^ (dv & (PQ - 1)))] = b[d];
+                for (int q = 0; q < 2; q++) {
+                    kc[q] = to_e4m3x4(x[0][i].get(4 * q) * ik, x[0][i].get(4 * q + 1) * ik, x[0][i].get(4 * q + 2) * ik, x[0][i].get(4 * q + 3) * ik);
+                    vc[i][q] = to_e4m3x4(x[1][i].get(4 * q) * iv, x[1][i].get(4 * q + 1) * iv, x[1][i].get(4 * q + 2) * iv, x[1][i].get(4 * q + 3) * iv);
+                    if (nan) kc[q] = 0x7f7f7f7fu;
+                }
+                if (tok < n) *reinterpret_cast<u32x2 *>(Kp + (size_t)(off + tok) * HD + 8 * dv) = kc;
+            }
+            // [4 tokens][8 dims] -> [8 dims][4 tokens]. Word (dim d, tokens 4 tq ..) of the tile sits at d * PQ + (tq ^ (d / 8 %
+            // PQ)): the lanes of a wave hold dims 8 apart, which would all share a bank.
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const uint32_t l01 = __builtin_amdgcn_perm(vc[1][q], vc[0][q], 0x05010400u), h01 = __builtin_amdgcn_perm(vc[1][q], vc[0][q], 0x07030602u);
+                const uint32_t l23 = __builtin_amdgcn_perm(vc[3][q], vc[2][q], 0x05010400u), h23 = __builtin_amdgcn_perm(vc[3][q], vc[2][q], 0x07030602u);
+                const uint32_t b[4] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
+                                       __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u)};
+#pragma unroll
+                for (int d = 0; d < 4; d++) tw[(8 * dv + 4 * q + d) * PQ + (tg ^ (dv & (PQ - 1)))] = b[d];
+            }
         }
         __syncthreads();
         const int whole = off == 0 ? n >> 4 : 0;                    // 16-token pieces that the run covers
@@ -352,12 +399,16 @@ static hipError_t launch_append_t(const AppendArgs &a, dim3 grid, int threads, h
 
 hipError_t launch_kv8_append(const void *k, const void *v, int src_dtype, long k_stride, long v_stride, const Kv8 &c,
                              const int *slots, int rows, unsigned *stats, hipStream_t st) {
-    AppendArgs a{k, v, k_stride, v_stride, c, slots, stats, rows, 1, 0};
+    AppendArgs a{k, v, k_stride, v_stride, c, slots, stats, rows, 1, 0, 0};
     while ((8 << a.lv) < c.HD) a.lv++;
     // A workgroup looks for runs among `win` rows. One row each while the rows are few (a decode step's rows are runs of
-    // one, and a window's runs are taken one after another); 16 for long prompts, where 15 of 16 would find none.
-    if ((long long)rows * c.NKV > 16384) a.win = 16;
-    const dim3 grid((unsigned)((rows + a.win - 1) / a.win), (unsigned)c.NKV);
+    // one, and a window's runs are taken one after another); more for prompts, where most workgroups would find none.
+    const long long units = (long long)rows * c.NKV;
+    a.win = units <= 4096 ? 1 : units <= 32768 ? 4 : 16;
+    a.windows = (rows - 1) / a.win + 1;
+    const long long wgs = ((long long)a.windows * c.NKV + 7) / 8 * 8;
+    if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)wgs);
     const int threads = c.page * c.HD / 32;
     switch (src_dtype) {
     case DT_FP32: return launch_append_t<DT_FP32>(a, grid, threads, st);

@@ -264,9 +264,29 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _i32(t, what, dev):
-    _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == dev, f"{what}: a contiguous int32 tensor on {dev} is wanted")
+def _i32(t, dev, what):
+    """Address of a contiguous int32 tensor on device number `dev`."""
+    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 tensor on device {dev} is wanted")
     return t.data_ptr()
+
+
+def _table(t, dev, B, what):
+    """Address, row stride and columns of a block table [B, cols] with contiguous rows."""
+    shape = t.shape
+    if t.dtype is not torch.int32 or t.get_device() != dev or len(shape) != 2 or shape[0] != B:
+        raise ValueError(f"{what}: table [{B}, cols] int32 on device {dev} is wanted")
+    stride = t.stride()
+    cols = shape[1]
+    if (cols > 1 and stride[1] != 1) or (B > 1 and stride[0] < cols):
+        raise ValueError(f"{what}: the rows of table have to be contiguous and apart")
+    return t.data_ptr(), stride[0] if B > 1 else cols, cols
+
+
+def _here(dev, what):
+    """`dev` is the current device, whose stream the call takes."""
+    if dev < 0 or dev != _get_device():
+        raise ValueError(f"{what}: the tensors are on {'the host' if dev < 0 else f'device {dev}'}, not on the current device")
 
 
 class KV8Cache:
@@ -283,7 +303,7 @@ class KV8Cache:
         _need(K.shape[2] in (16, 32, 64) and K.shape[3] in (128, 256, 512), "KV8Cache: pages of 16, 32 or 64 tokens and head dims of 128, 256 or 512 are wanted")
         self.K, self.V, self.Ks, self.Vs = K, V, Ks, Vs
         self.pages, self.NKV, self.page, self.HD = K.shape
-        self.device = K.device
+        self.device, self._dev = K.device, K.get_device()
         self._c = _KV8(K.data_ptr(), V.data_ptr(), Ks.data_ptr(), Vs.data_ptr(), self.pages, self.page, self.NKV, self.HD)
         self._p = ctypes.addressof(self._c)
 
@@ -295,38 +315,35 @@ class KV8Cache:
                    torch.ones(pages, NKV, device=device))
 
 
-def _on_device(dev, what):
-    _need(dev.type == "cuda" and dev.index == _get_device(), f"{what}: the tensors are on {dev}, which is not the current device")
-
-
 def kv8_plan(ctx, add, page, table, free_pages, free_in, free_out, cu, slots, status):
     """Block tables and slot maps of a step (dgx_kv8_plan): ctx, add [B], table [B, cols] (rows may be strided), free_pages
     [cap], free_in / free_out / status [1], cu [B + 1], slots [rows], all int32. status tells whether the step took its
     pages; nothing is checked on the host."""
-    dev, B = ctx.device, ctx.shape[0]
-    _on_device(dev, "kv8_plan")
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.device == dev and table.shape[0] == B and
-          (table.stride(1) == 1 or table.shape[1] <= 1), "kv8_plan: table [B, cols] int32 with contiguous rows is wanted")
-    _need(add.shape[0] == B and cu.shape[0] == B + 1 and ctx.dim() == add.dim() == cu.dim() == 1, "kv8_plan: ctx and add [B], cu [B + 1] are wanted")
-    _need(free_in.numel() >= 1 and free_out.numel() >= 1 and status.numel() >= 1, "kv8_plan: free_in, free_out and status hold one number each")
-    stride = table.stride(0) if B > 1 else table.shape[1]
-    _need(stride >= table.shape[1], "kv8_plan: the rows of table overlap")
-    _ck(lib().dgx_kv8_plan(_i32(ctx, "ctx", dev), _i32(add, "add", dev), B, page, table.data_ptr(), stride, table.shape[1],
-                           _i32(free_pages, "free_pages", dev), free_pages.numel(), _i32(free_in, "free_in", dev),
-                           _i32(free_out, "free_out", dev), _i32(cu, "cu", dev), _i32(slots, "slots", dev), slots.numel(),
-                           _i32(status, "status", dev), _stream()), "dgx_kv8_plan")
+    dev, B = ctx.get_device(), ctx.numel()
+    _here(dev, "kv8_plan")
+    tab, stride, cols = _table(table, dev, B, "kv8_plan")
+    if add.numel() != B or cu.numel() != B + 1:
+        raise ValueError("kv8_plan: ctx and add [B], cu [B + 1] are wanted")
+    if not (free_in.numel() and free_out.numel() and status.numel()):
+        raise ValueError("kv8_plan: free_in, free_out and status hold one number each")
+    _ck(lib().dgx_kv8_plan(_i32(ctx, dev, "ctx"), _i32(add, dev, "add"), B, page, tab, stride, cols, _i32(free_pages, dev, "free_pages"),
+                           free_pages.numel(), _i32(free_in, dev, "free_in"), _i32(free_out, dev, "free_out"), _i32(cu, dev, "cu"),
+                           _i32(slots, dev, "slots"), slots.numel(), _i32(status, dev, "status"), _stream()), "dgx_kv8_plan")
 
 
 def kv8_append(k, v, cache, slots):
     """Append rows k, v [rows, NKV, HD] (fp32, f16 or bf16; rows may be strided) at slots [rows] (dgx_kv8_append)."""
-    dev, rows = cache.device, slots.shape[0]
-    _on_device(dev, "kv8_append")
-    for t in (k, v):
-        _need(tuple(t.shape) == (rows, cache.NKV, cache.HD) and t.dtype == k.dtype and t.dtype in _DT and t.device == dev and
-              t.stride(2) == 1 and t.stride(1) == cache.HD, "kv8_append: k and v [rows, NKV, HD] of one type with contiguous rows are wanted")
+    dev, rows = cache._dev, slots.numel()
+    _here(dev, "kv8_append")
+    shape, ks, vs = (rows, cache.NKV, cache.HD), k.stride(), v.stride()
+    dt = _DT.get(k.dtype)
+    if k.shape != shape or v.shape != shape or dt is None or v.dtype is not k.dtype or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"kv8_append: k and v {list(shape)} of one type (fp32, f16, bf16) on the cache's device are wanted")
     row = cache.NKV * cache.HD
-    _ck(lib().dgx_kv8_append(k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0) if rows > 1 else row, v.stride(0) if rows > 1 else row,
-                             cache._p, _i32(slots, "slots", dev), rows, _stream()), "dgx_kv8_append")
+    if ks[2] != 1 or vs[2] != 1 or (cache.NKV > 1 and (ks[1] != cache.HD or vs[1] != cache.HD)) or (rows > 1 and min(ks[0], vs[0]) < row):
+        raise ValueError("kv8_append: the rows of k and v have to be contiguous and apart")
+    _ck(lib().dgx_kv8_append(k.data_ptr(), v.data_ptr(), dt, ks[0] if rows > 1 else row, vs[0] if rows > 1 else row, cache._p,
+                             _i32(slots, dev, "slots"), rows, _stream()), "dgx_kv8_append")
 
 
 def attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk=0, window=0, tree=False):
@@ -339,27 +356,31 @@ def attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk=0, window=0, tree
 def attn_kv8(Q, cache, table, ctx, O, T, max_pos, cu=None, anc=None, chunk=0, ws=None, scale=0.0, window=0, lse=None):
     """Attention over the paged 8-bit cache (dgx_attn_kv8): Q, O [rows, NQ, HD], table [B, cols] and ctx [B] int32, cu [B + 1]
     (None: T rows each), anc [rows] int32, ws a uint8 tensor of attn_kv8_workspace bytes (allocated here when None)."""
-    dev, B, rows, NQ = cache.device, ctx.shape[0], Q.shape[0], Q.shape[1]
-    _on_device(dev, "attn_kv8")
-    _need(Q.dim() == 3 and Q.shape[2] == cache.HD and Q.shape == O.shape and Q.is_contiguous() and O.is_contiguous() and
-          Q.device == dev and O.device == dev and Q.dtype in (torch.float16, torch.bfloat16) and O.dtype in _DT,
-          "attn_kv8: contiguous Q (f16, bf16) and O [rows, NQ, HD] on the cache's device are wanted")
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.device == dev and table.shape[0] == B and
-          (table.stride(1) == 1 or table.shape[1] <= 1), "attn_kv8: table [B, cols] int32 with contiguous rows is wanted")
-    _need(table.shape[1] > max_pos // cache.page, "attn_kv8: table has too few columns for max_pos")
-    _need(cu is None or cu.shape[0] == B + 1, "attn_kv8: cu [B + 1] is wanted")
-    _need(anc is None or anc.numel() == rows, "attn_kv8: anc [rows] is wanted")
-    _need(lse is None or (lse.numel() == rows * NQ and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev),
-          "attn_kv8: lse [rows, NQ] fp32 is wanted")
+    dev, B, shape = cache._dev, ctx.numel(), Q.shape
+    _here(dev, "attn_kv8")
+    qt, ot = _DT.get(Q.dtype), _DT.get(O.dtype)
+    if (len(shape) != 3 or shape[2] != cache.HD or O.shape != shape or not qt or ot is None or Q.get_device() != dev or
+            O.get_device() != dev or not Q.is_contiguous() or not O.is_contiguous()):
+        raise ValueError("attn_kv8: contiguous Q (f16, bf16) and O [rows, NQ, HD] on the cache's device are wanted")
+    rows, NQ = shape[0], shape[1]
+    tab, stride, cols = _table(table, dev, B, "attn_kv8")
+    if cols <= max_pos // cache.page:
+        raise ValueError("attn_kv8: table has too few columns for max_pos")
+    if cu is not None and cu.numel() != B + 1:
+        raise ValueError("attn_kv8: cu [B + 1] is wanted")
+    if anc is not None and anc.numel() != rows:
+        raise ValueError("attn_kv8: anc [rows] is wanted")
+    if lse is not None and (lse.numel() != rows * NQ or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != dev):
+        raise ValueError("attn_kv8: lse [rows, NQ] fp32 is wanted")
     if ws is None:
         ws = torch.empty(attn_kv8_workspace(B, T, rows, NQ, cache.NKV, cache.HD, max_pos, chunk, window, anc is not None),
-                         dtype=torch.uint8, device=dev)
-    _need(ws.is_contiguous() and ws.device == dev, "attn_kv8: a contiguous ws on the cache's device is wanted")
-    stride = table.stride(0) if B > 1 else table.shape[1]
-    _ck(lib().dgx_attn_kv8(Q.data_ptr(), _DT[Q.dtype], cache._p, table.data_ptr(), stride, O.data_ptr(), _DT[O.dtype], _ptr(lse),
-                           B, T, rows, NQ, _i32(ctx, "ctx", dev), None if cu is None else _i32(cu, "cu", dev),
-                           None if anc is None else _i32(anc, "anc", dev), max_pos, chunk, ws.data_ptr(),
-                           ws.numel() * ws.element_size(), _stream(), float(scale), window), "dgx_attn_kv8")
+                         dtype=torch.uint8, device=cache.device)
+    elif ws.dtype is not torch.uint8 or ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError("attn_kv8: a contiguous uint8 ws on the cache's device is wanted")
+    _ck(lib().dgx_attn_kv8(Q.data_ptr(), qt, cache._p, tab, stride, O.data_ptr(), ot, None if lse is None else lse.data_ptr(), B, T, rows,
+                           NQ, _i32(ctx, dev, "ctx"), None if cu is None else _i32(cu, dev, "cu"),
+                           None if anc is None else _i32(anc, dev, "anc"), max_pos, chunk, ws.data_ptr(), ws.numel(), _stream(),
+                           scale, window), "dgx_attn_kv8")
 
 
 def timing(on):
