@@ -84,7 +84,7 @@ struct Kv8DecCfg {
     static constexpr int PSTR = SK + 8;                // P row, likewise
     static constexpr size_t LDS_Q = (size_t)RR * QSTR * 2, LDS_P = (size_t)RR * PSTR * 2;
     static constexpr size_t LDS = LDS_Q + LDS_P + (size_t)NW * RR * 4;
-    static constexpr int OCC = NT == 1 ? 3 : 2;        // waves per SIMD that the registers are held to
+    static constexpr int OCC = NT > 1 ? 2 : HD == 256 ? 3 : 4;   // waves per SIMD that the registers are held to
 };
 
 constexpr float kv8_head = 6.f, kv8_move = 14.f;       // the reference lies 2^6 under its maximum and moves above 2^14
@@ -118,31 +118,27 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     const int last_col = p.max_pos >> kc.lp;
     auto safe = [&](int id) { return (unsigned)id < (unsigned)kc.pages ? id : 0; };
 
-    // Pages of a step's eight 16-key pieces, and the scales of the wave's own KT: uniform, loaded a step or two ahead.
-    struct Ids { int p[8]; };
-    auto ids_of = [&](int s) {
-        Ids q;
+    // A step's pages and scales, loaded a step or two ahead: of the wave's own KT 16-key pieces through the scalar cache, of
+    // the lane's V columns (the pieces g and 4 + g) as vectors. (Not picked from one list of all eight: the compiler puts a list
+    // that is indexed by wave into memory, and reading it back waits for every load in flight.)
+    struct Own { int id[KT]; };
+    struct Scales { float k[KT], v[KT]; };
+    auto own_ids = [&](int s) {
+        Own q;
 #pragma unroll
-        for (int i = 0; i < 8; i++) q.p[i] = scalar_load(tab + min((SK * s + 16 * i) >> kc.lp, last_col));
+        for (int t = 0; t < KT; t++) q.id[t] = scalar_load(tab + min((SK * s + 16 * (KT * wave + t)) >> kc.lp, last_col));
         return q;
     };
-    struct Scales { float k[KT], v[KT]; bool ok[KT], all; };
-    auto scales_of = [&](const Ids &q) {
+    auto scales_of = [&](const Own &q) {
         Scales r;
-        r.all = true;
-#pragma unroll
-        for (int i = 0; i < 8; i++) r.all &= (unsigned)q.p[i] < (unsigned)kc.pages;
 #pragma unroll
         for (int t = 0; t < KT; t++) {
-            int id = q.p[t];
-#pragma unroll
-            for (int w = 1; w < NW; w++) id = wave == w ? q.p[KT * w + t] : id;
-            const size_t cell = (size_t)safe(id) * kc.NKV + h;
-            r.ok[t] = (unsigned)id < (unsigned)kc.pages;
+            const size_t cell = (size_t)safe(q.id[t]) * kc.NKV + h;
             r.k[t] = scalar_load(kc.Ks + cell); r.v[t] = scalar_load(kc.Vs + cell);
         }
         return r;
     };
+    auto v_id = [&](int s, int k) { return tab[min((SK * s + 64 * k + 16 * g) >> kc.lp, last_col)]; };
     const size_t head_bytes = (size_t)page * HD;
     auto fetch = [](const uint8_t *q) {
         if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(q));
@@ -150,39 +146,43 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     };
     u32x4 kr[KT][DC], vr[2][DB];
     const unsigned klane = (unsigned)(ln * HD + 16 * g);
-    auto load_k = [&](int s, const Ids &q) {                           // tile t: key 16 (KT wave + t) + ln of the step
+    auto load_k = [&](int s, const Own &q) {                           // tile t: key 16 (KT wave + t) + ln of the step
 #pragma unroll
         for (int t = 0; t < KT; t++) {
-            int id = q.p[t];
-#pragma unroll
-            for (int w = 1; w < NW; w++) id = wave == w ? q.p[KT * w + t] : id;
-            const uint8_t *b = kc.K + ((size_t)safe(id) * kc.NKV + h) * head_bytes + (size_t)((SK * s + 16 * (KT * wave + t)) & (page - 1)) * HD;
+            const uint8_t *b = kc.K + ((size_t)safe(q.id[t]) * kc.NKV + h) * head_bytes + (size_t)((SK * s + 16 * (KT * wave + t)) & (page - 1)) * HD;
 #pragma unroll
             for (int d = 0; d < DC; d++) kr[t][d] = fetch(b + (klane + 64 * d));
         }
     };
-    const unsigned vlane = (unsigned)((wave * (HD / NW) + ln) * page);
-    auto load_v = [&](int s, const Ids &q) {                           // dims of the wave, 16 tokens from 64 k + 16 g of the step
+    const unsigned vlane = (unsigned)((wave * (HD / NW) + ln) * page + ((16 * g) & (page - 1)));
+    auto load_v = [&](int k, int id) {                                 // dims of the wave, 16 tokens from 64 k + 16 g of the step
+        const uint8_t *b = kc.V + (size_t)(unsigned)(safe(id) * kc.NKV + h) * head_bytes + vlane;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int id = g < 2 ? (g ? safe(q.p[4 * k + 1]) : safe(q.p[4 * k])) : g == 2 ? safe(q.p[4 * k + 2]) : safe(q.p[4 * k + 3]);
-            const uint8_t *b = kc.V + (size_t)(unsigned)(id * kc.NKV + h) * head_bytes + (vlane + ((16 * g) & (page - 1)));
-#pragma unroll
-            for (int d = 0; d < DB; d++) vr[k][d] = fetch(b + 16 * d * page);
-        }
-        (void)s;
+        for (int d = 0; d < DB; d++) vr[k][d] = fetch(b + 16 * d * page);
     };
 
     const int s1 = j_hi > j_lo ? (j_hi - 1) / SK : -1;
     int s = j_lo / SK;
-    Ids nxt{};
+    Own nxt{};
     Scales sn{};
+    bool okn = true;                                                   // the wave's pages are in the pool
+    int vi0 = 0, vi1 = 0, vn0 = 0, vn1 = 0;                            // V pages of this step and of the next one
+    auto own_ok = [&](const Own &q) {
+        bool r = true;
+#pragma unroll
+        for (int t = 0; t < KT; t++) r &= (unsigned)q.id[t] < (unsigned)kc.pages;
+        return r;
+    };
+    Own cur{};
     if (s <= s1) {
-        const Ids q = ids_of(s);
-        nxt = ids_of(min(s + 1, s1));
-        load_k(s, q);
-        load_v(s, q);
-        sn = scales_of(q);
+        cur = own_ids(s);
+        vi0 = v_id(s, 0); vi1 = v_id(s, 1);
+        nxt = own_ids(min(s + 1, s1));
+        load_k(s, cur);
+        load_v(0, vi0); load_v(1, vi1);
+        vn0 = v_id(min(s + 1, s1), 0); vn1 = v_id(min(s + 1, s1), 1);
+        sn = scales_of(cur);
+        okn = own_ok(cur);
     }
     // Q rows, zeros past the last.
     uint16_t *qs = reinterpret_cast<uint16_t *>(smem), *ps = reinterpret_cast<uint16_t *>(smem + Cf::LDS_Q);
@@ -218,6 +218,14 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     for (; s <= s1; s++) {
         const int j0 = SK * s, jw = j0 + 16 * KT * wave;
         const Scales sc = sn;
+        const Own now = cur;
+        const bool pages_ok = okn;
+        if (s < s1) {                                                  // (these wait together with the K loads of this step)
+            cur = nxt;
+            sn = scales_of(cur);
+            okn = own_ok(cur);
+            nxt = own_ids(min(s + 2, s1));
+        }
         f32x4 st[KT][NT];
 #pragma unroll
         for (int t = 0; t < KT; t++)
@@ -240,15 +248,11 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
                 for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k1[t], q1, st[t][nt]);
             }
         }
-        Ids cur = nxt;
+        int vf0 = 0, vf1 = 0;
         if (s < s1) {
+            vf0 = v_id(min(s + 2, s1), 0); vf1 = v_id(min(s + 2, s1), 1);
             load_k(s + 1, cur);
-            sn = scales_of(cur);
-            nxt = ids_of(min(s + 2, s1));
         }
-        bool pages_ok = true;
-#pragma unroll
-        for (int t = 0; t < KT; t++) pages_ok &= sc.ok[t];
         const bool full = pages_ok && jw >= j_lo && jw + 16 * KT <= j_hi && jw >= lo_max && jw + 16 * KT - 1 <= pos_min;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
 #pragma unroll
                 for (int i = 0; i < 4; i++) st[t][nt][i] = __builtin_fmaf(st[t][nt][i], kf, ev);
                 if (!full) {
-                    const int kb = jw + 16 * t + 4 * g, kl = max(j_lo, win_lo(rpos[nt], p.window)) - kb, kh = sc.ok[t] ? min(j_hi - 1, rpos[nt]) - kb : -1;
+                    const int kb = jw + 16 * t + 4 * g, kl = max(j_lo, win_lo(rpos[nt], p.window)) - kb, kh = (unsigned)now.id[t] < (unsigned)kc.pages ? min(j_hi - 1, rpos[nt]) - kb : -1;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         bool out = (i < kl) | (i > kh);
@@ -300,12 +304,12 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
             }
         }
         __syncthreads();
-        if (!sc.all || j0 < j_lo || j0 + SK > j_hi) {                  // bytes that are no token of the request's: any code, NaN too
+        const bool vok0 = (unsigned)vi0 < (unsigned)kc.pages, vok1 = (unsigned)vi1 < (unsigned)kc.pages;
+        if (j0 < j_lo || j0 + SK > j_hi || __any(!(vok0 & vok1))) {    // bytes that are no token of the request's: any code, NaN too
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                // (a page outside the pool was read as page 0, whose codes may be NaN: its id is gone here, the table is read again)
-                const int jb = j0 + 64 * k + 16 * g, id = tab[min(jb >> kc.lp, last_col)];
-                const int k0 = (unsigned)id < (unsigned)kc.pages ? max(j_lo - jb, 0) : 16, k1 = min(j_hi - jb, 16);
+                const int jb = j0 + 64 * k + 16 * g;
+                const int k0 = (k ? vok1 : vok0) ? max(j_lo - jb, 0) : 16, k1 = min(j_hi - jb, 16);
                 u32x4 keep;
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
@@ -334,7 +338,8 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
                 for (int nt = 0; nt < NT; nt++) acc[nt][d] = mfma16<true>(v1, pf[nt][1], acc[nt][d]);
             }
         }
-        if (s < s1) load_v(s + 1, cur);
+        if (s < s1) { load_v(0, vn0); load_v(1, vn1); }
+        vi0 = vn0; vi1 = vn1; vn0 = vf0; vn1 = vf1;
     }
 
     // Row sums over the waves, in their order; m is the same in all.

@@ -107,25 +107,19 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     const int page = kc.page, last_col = p.max_pos >> kc.lp;
     const int *tab = p.table + (size_t)seq * p.table_stride;
     auto safe = [&](int id) { return (unsigned)id < (unsigned)kc.pages ? id : 0; };
-    // Pages of a step's four 16-key pieces, and the scales of the wave's two: all uniform, loaded a step or two ahead.
-    struct Ids { int p[4]; };
+    // A step's pages and scales, loaded a step or two ahead: of the wave's two 16-key pieces and of its K loads through the
+    // scalar cache, of the lane's V loads as a vector. (Not picked from one list of all four: the compiler puts a list that is
+    // indexed by wave into memory, and reading it back waits for every load in flight.)
+    auto piece_id = [&](int s, int piece) { return scalar_load(tab + min((64 * s + 16 * piece) >> kc.lp, last_col)); };
+    struct Ids { int a, b, k, v; };
     auto ids_of = [&](int s) {
-        Ids q;
-#pragma unroll
-        for (int i = 0; i < 4; i++) q.p[i] = scalar_load(tab + min((64 * s + 16 * i) >> kc.lp, last_col));
-        return q;
+        return Ids{piece_id(s, 2 * kg), piece_id(s, 2 * kg + 1), piece_id(s, wave >> 1), tab[min((64 * s + 16 * ((lane & 3) ^ ((lane >> 4) & 3))) >> kc.lp, last_col)]};
     };
-    struct Scales { float k[2], v[2]; bool ok[2]; };
+    struct Scales { float ka, kb, va, vb; bool oka, okb; };
     auto scales_of = [&](const Ids &q) {
-        Scales r;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int id = kg ? q.p[2 + i] : q.p[i];
-            const size_t cell = (size_t)safe(id) * kc.NKV + h;
-            r.ok[i] = (unsigned)id < (unsigned)kc.pages;
-            r.k[i] = scalar_load(kc.Ks + cell); r.v[i] = scalar_load(kc.Vs + cell);
-        }
-        return r;
+        const size_t ca = (size_t)safe(q.a) * kc.NKV + h, cb = (size_t)safe(q.b) * kc.NKV + h;
+        return Scales{scalar_load(kc.Ks + ca), scalar_load(kc.Ks + cb), scalar_load(kc.Vs + ca), scalar_load(kc.Vs + cb),
+                      (unsigned)q.a < (unsigned)kc.pages, (unsigned)q.b < (unsigned)kc.pages};
     };
 
     // Step loads. K slot S = (wave NLD + u) 64 + lane: key S / SLOTS, 16-byte column (S % SLOTS) ^ kf(key); a wave's keys lie
@@ -142,18 +136,16 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
     const size_t head_bytes = (size_t)page * HD;
     auto issue = [&](int s, const Ids &q) {
         const unsigned st = lds0 + (unsigned)(s & 1) * Cf::STAGE + (unsigned)wave * NLD * 1024;
-        const int kid = safe(kpiece == 0 ? q.p[0] : kpiece == 1 ? q.p[1] : kpiece == 2 ? q.p[2] : q.p[3]);
-        const uint8_t *kb = kc.K + ((size_t)kid * kc.NKV + h) * head_bytes + (size_t)((64 * s + 16 * kpiece) & (page - 1)) * HD;
-        const int vid = vpiece < 2 ? (vpiece ? safe(q.p[1]) : safe(q.p[0])) : vpiece == 2 ? safe(q.p[2]) : safe(q.p[3]);
-        const uint8_t *vb = kc.V + ((size_t)(unsigned)(vid * kc.NKV + h)) * head_bytes + (unsigned)((wave * NLD * 16 + (lane >> 2)) * page + ((64 * s + 16 * vpiece) & (page - 1)));
+        const uint8_t *kb = kc.K + ((size_t)safe(q.k) * kc.NKV + h) * head_bytes + (size_t)((64 * s + 16 * kpiece) & (page - 1)) * HD;
+        const uint8_t *vb = kc.V + (size_t)(unsigned)(safe(q.v) * kc.NKV + h) * head_bytes + (unsigned)((wave * NLD * 16 + (lane >> 2)) * page + ((64 * s + 16 * vpiece) & (page - 1)));
 #pragma unroll
         for (int u = 0; u < NLD; u++) {
             load_to_lds16(kb + koff[u], st + u * 1024);
             load_to_lds16(vb + 16 * u * page, st + Cf::HALF + u * 1024);
         }
     };
-    Ids nxt{{0, 0, 0, 0}};
-    Scales sn{{1.f, 1.f}, {1.f, 1.f}, {true, true}};
+    Ids nxt{0, 0, 0, 0};
+    Scales sn{1.f, 1.f, 1.f, 1.f, true, true};
     if (s_lo <= s_hi) {
         const Ids q = ids_of(s_lo);
         nxt = ids_of(min(s_lo + 1, s_hi));
@@ -238,10 +230,10 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
                 for (int rb = 0; rb < RB; rb++) st[t][rb] = mfma16<F16>(k1, qop[rb][2 * d + 1], st[t][rb]);
             }
         }
-        const bool up = g >= 2, ok = up ? sc.ok[1] : sc.ok[0];         // the lane's 8 keys are in piece g / 2 of the wave's
-        const float f = (up ? sc.k[1] : sc.k[0]) * a.sl2, ev = up ? (float)exp_of(sc.v[1]) : (float)exp_of(sc.v[0]);
-        const float iv = up ? pow2i(-exp_of(sc.v[1])) : pow2i(-exp_of(sc.v[0]));
-        const bool part = jw < j_lo || jw + 32 > j_hi || !(sc.ok[0] & sc.ok[1]);
+        const bool up = g >= 2, ok = up ? sc.okb : sc.oka;             // the lane's 8 keys are in piece g / 2 of the wave's
+        const float f = (up ? sc.kb : sc.ka) * a.sl2, ev = up ? (float)exp_of(sc.vb) : (float)exp_of(sc.va);
+        const float iv = up ? pow2i(-exp_of(sc.vb)) : pow2i(-exp_of(sc.va));
+        const bool part = jw < j_lo || jw + 32 > j_hi || !(sc.oka & sc.okb);
         u32x4 pf[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
