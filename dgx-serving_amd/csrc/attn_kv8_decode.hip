@@ -263,13 +263,14 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
 #pragma unroll
                 for (int i = 0; i < 4; i++) st[t][nt][i] = __builtin_fmaf(st[t][nt][i], kf, ev);
                 if (!full) {
-                    const int kb = jw + 16 * t + 4 * g, kl = max(j_lo, win_lo(rpos[nt], p.window)) - kb, kh = (unsigned)now.id[t] < (unsigned)kc.pages ? min(j_hi - 1, rpos[nt]) - kb : -1;
+                    const int kb = jw + 16 * t + 4 * g, kl = max(j_lo, win_lo(rpos[nt], p.window)) - kb;
+                    const int kh = (unsigned)now.id[t] < (unsigned)kc.pages ? min(j_hi - 1, rpos[nt]) - kb : -1;
+                    // Bit i: key kb + i is hidden by the tree (tokens from 32 on, and those whose bit is not set).
+                    const int d = kb - p0;
+                    const uint32_t tree = !p.anc ? 0u : ~(uint32_t)((d <= -32 ? ~0ull : d < 0 ? ((uint64_t)ranc[nt] << -d) | ((1ull << -d) - 1) : d < 32 ? (uint64_t)(ranc[nt] >> d) : 0ull));
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        bool out = (i < kl) | (i > kh);
-                        if (p.anc) { const int d = kb + i - p0; out |= (d >= 0) & ((d >= 32) | !((ranc[nt] >> (d & 31)) & 1u)); }
-                        if (out) st[t][nt][i] = kNegInf;
-                    }
+                    for (int i = 0; i < 4; i++)
+                        if ((i < kl) | (i > kh) | (bool)((tree >> i) & 1u)) st[t][nt][i] = kNegInf;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[t][nt][i]);
@@ -290,14 +291,12 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
 #pragma unroll
                 for (int d = 0; d < DB; d++) acc[nt][d] *= al;
             }
+            const float mz = m[nt] == kNegInf ? 0.f : m[nt];           // (no key yet: every 2^(-inf) is 0)
 #pragma unroll
             for (int t = 0; t < KT; t++) {
                 float pv[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float x = st[t][nt][i];
-                    pv[i] = full ? fast_exp2(x - m[nt]) : x == kNegInf ? 0.f : fast_exp2(x - m[nt]);   // (a row without a key yet: m = -inf)
-                }
+                for (int i = 0; i < 4; i++) pv[i] = fast_exp2(st[t][nt][i] - mz);
                 l[nt] = __builtin_fmaf((pv[0] + pv[1]) + (pv[2] + pv[3]), pow2i(-exp_of(sc.v[t])), l[nt]);
                 *reinterpret_cast<u32x2 *>(ps + (16 * nt + ln) * Cf::PSTR + 16 * (KT * wave + t) + 4 * g) =
                     u32x2{pack2<true>(pv[0], pv[1]), pack2<true>(pv[2], pv[3])};

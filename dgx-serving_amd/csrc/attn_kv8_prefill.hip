@@ -258,11 +258,11 @@ __global__ void __launch_bounds__(512) kv8_prefill_kernel(const Kv8PrefArgs a) {
 #pragma unroll
                 for (int d = 0; d < DB; d++) acc[rb][d] *= al;
             }
+            const float mz = m[rb] == kNegInf ? 0.f : m[rb];           // (no key yet: every 2^(-inf) is 0)
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                if (full) tv[i] = fast_exp2(tv[i] - m[rb]);
-                else tv[i] = tv[i] == kNegInf ? 0.f : fast_exp2(tv[i] - m[rb]);
+                tv[i] = fast_exp2(tv[i] - mz);
                 sum += tv[i];
             }
             l[rb] = __builtin_fmaf(sum, iv, l[rb]);
