@@ -27,6 +27,7 @@
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 namespace dgx {
 
@@ -75,16 +76,20 @@ __device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M,
 template <int HD, int NT>
 struct Kv8DecCfg {
     static constexpr int SK = 128;                     // keys of a step
-    static constexpr int NW = HD == 512 ? 8 : 4;       // waves
+    static constexpr int NW = HD == 512 && NT > 1 ? 8 : 4;   // waves (8: registers)
     static constexpr int KT = SK / 16 / NW;            // 16-key tiles of a wave
     static constexpr int RR = 16 * NT;                 // query rows
     static constexpr int DC = HD / 64;                 // 64-dim pieces of a key (one 16-byte load per lane each)
     static constexpr int DB = HD / NW / 16;            // 16-dim output blocks of a wave
     static constexpr int QSTR = HD + 8;                // Q row in LDS: 16 rows on distinct bank quads
     static constexpr int PSTR = SK + 8;                // P row, likewise
-    static constexpr size_t LDS_Q = (size_t)RR * QSTR * 2, LDS_P = (size_t)RR * PSTR * 2;
-    static constexpr size_t LDS = LDS_Q + LDS_P + (size_t)NW * RR * 4;
-    static constexpr int OCC = NT > 1 ? 2 : HD == 256 ? 3 : 4;   // waves per SIMD that the registers are held to
+    // K through LDS (see load_k): a unit of 16 keys x 64 UD dims at a time, in a place of each wave's own.
+    static constexpr bool KLDS = NT == 1 || (NT == 2 && HD <= 256);
+    static constexpr int UD = DC < 4 ? DC : 4;
+    static constexpr size_t LDS_Q = (size_t)RR * QSTR * 2, LDS_P = (size_t)RR * PSTR * 2, LDS_K = KLDS ? (size_t)NW * 16 * 64 * UD : 0;
+    static constexpr size_t LDS_R = (size_t)NW * RR * 4;
+    static constexpr size_t LDS = LDS_Q + LDS_P + LDS_R + LDS_K;
+    static constexpr int OCC = NT > 1 || HD == 512 ? 2 : HD == 256 ? 3 : 4;   // waves per SIMD that the registers are held to
 };
 
 constexpr float kv8_head = 6.f, kv8_move = 14.f;       // the reference lies 2^6 under its maximum and moves above 2^14
@@ -94,11 +99,12 @@ template <int HD, int NT, bool F16, bool STREAM>
 __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, NT>::OCC)) kv8_decode_kernel(const Kv8DecArgs a) {
     using Cf = Kv8DecCfg<HD, NT>;
     constexpr int NW = Cf::NW, KT = Cf::KT, DC = Cf::DC, DB = Cf::DB, SK = Cf::SK;
+    constexpr bool KLDS = Cf::KLDS;
     extern __shared__ __align__(16) unsigned char smem[];
     const Kv8Problem &p = a.p;
     const Kv8 &kc = p.c;
     // Workgroups of one (chunk, KV head) and different row groups read the same keys: 8 apart, on one XCD.
-    const int unit = (int)(blockIdx.x / (8 * a.nrg)) * 8 + (int)(blockIdx.x & 7), rg = (int)(blockIdx.x >> 3) % a.nrg;
+    const int unit = (int)(blockIdx.x / (8 * a.nrg)) * 8 + (int)(blockIdx.x & 7), rg = a.nrg - 1 - (int)(blockIdx.x >> 3) % a.nrg;
     int seq, c, lo, hi;
     if (!kv8_find(p, a.C, a.Cm, a.direct, unit / kc.NKV, seq, c, lo, hi)) return;
     seq = __builtin_amdgcn_readfirstlane(seq); c = __builtin_amdgcn_readfirstlane(c);
@@ -108,12 +114,15 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     kv8_rows(p, seq, row0, nr);
     row0 = __builtin_amdgcn_readfirstlane(row0); nr = __builtin_amdgcn_readfirstlane(nr);
     const int rho0 = rg * Cf::RR, nrows = min(nr * G - rho0, Cf::RR);
-    const int j_lo = max(c * a.C, lo), j_hi = min(hi - c * a.C, a.C) + c * a.C;
-    if (nrows <= 0 || (j_lo >= j_hi && !a.direct)) return;
+    if (nrows <= 0) return;
+    // Keys of the chunk that some row of this group attends.
+    const int p0 = scalar_load(p.ctx + seq), t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
+    const int j_lo = max(c * a.C, win_lo(p0 + t_a, p.window)), j_hi = min(min(hi, p0 + t_b + 1) - c * a.C, a.C) + c * a.C;
+    if (j_lo >= j_hi && !a.direct) return;
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, ln = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int p0 = scalar_load(p.ctx + seq), page = kc.page;
+    const int page = kc.page;
     const int *tab = p.table + (size_t)seq * p.table_stride;
     const int last_col = p.max_pos >> kc.lp;
     auto safe = [&](int id) { return (unsigned)id < (unsigned)kc.pages ? id : 0; };
@@ -145,13 +154,24 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
         else return *reinterpret_cast<const u32x4 *>(q);
     };
     u32x4 kr[KT][DC], vr[2][DB];
-    const unsigned klane = (unsigned)(ln * HD + 16 * g);
-    auto load_k = [&](int s, const Own &q) {                           // tile t: key 16 (KT wave + t) + ln of the step
+    // K of the wave, tile t: key 16 (KT wave + t) + ln of the step. A fragment is 16 dims of each of 16 keys: loaded as such,
+    // a load touches 64 bytes of 16 rows and takes five times as long to issue as one of whole rows (32 of them 1.1 us a step
+    // at HD 256, more than the rest of a step that waits for nothing). With few rows K is therefore loaded in whole rows
+    // and goes through LDS, 16-byte slots XOR-swizzled by the key; with more, Q takes the LDS and its bandwidth.
+    constexpr int UD = Cf::UD;
+    auto kswz = [](int key) { return UD == 4 ? key : key >> 1; };
+    unsigned klane[KLDS ? UD : 1];
+#pragma unroll
+    for (int u = 0; u < (KLDS ? UD : 1); u++) {
+        const int S = 64 * u + lane;
+        klane[u] = KLDS ? (unsigned)(S / (4 * UD) * HD + S % (4 * UD) * 16) : (unsigned)(ln * HD + 16 * g);
+    }
+    auto load_k = [&](int s, const Own &q) {
 #pragma unroll
         for (int t = 0; t < KT; t++) {
             const uint8_t *b = kc.K + ((size_t)safe(q.id[t]) * kc.NKV + h) * head_bytes + (size_t)((SK * s + 16 * (KT * wave + t)) & (page - 1)) * HD;
 #pragma unroll
-            for (int d = 0; d < DC; d++) kr[t][d] = fetch(b + (klane + 64 * d));
+            for (int d = 0; d < DC; d++) kr[t][d] = fetch(b + (KLDS ? klane[d % UD] + 64 * UD * (d / UD) : klane[0] + 64 * d));
         }
     };
     const unsigned vlane = (unsigned)((wave * (HD / NW) + ln) * page + ((16 * g) & (page - 1)));
@@ -187,6 +207,14 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     // Q rows, zeros past the last.
     uint16_t *qs = reinterpret_cast<uint16_t *>(smem), *ps = reinterpret_cast<uint16_t *>(smem + Cf::LDS_Q);
     float *red = reinterpret_cast<float *>(smem + Cf::LDS_Q + Cf::LDS_P);
+    unsigned char *ks = smem + Cf::LDS_Q + Cf::LDS_P + Cf::LDS_R + (size_t)wave * 16 * 64 * UD;
+    unsigned kw[KLDS ? UD : 1];                                        // where the lane's loads go in a unit, and its fragment's row
+#pragma unroll
+    for (int u = 0; u < (KLDS ? UD : 1); u++) {
+        const int S = 64 * u + lane, key = S / (4 * UD);
+        kw[u] = (unsigned)(key * 64 * UD + ((S % (4 * UD) ^ kswz(key)) << 4));
+    }
+    const unsigned kfrag = (unsigned)(ln * 64 * UD + ((g ^ kswz(ln)) << 4));
     for (int i = tid; i < Cf::RR * (HD / 8); i += NW * 64) {
         const int R = i / (HD / 8), rho = rho0 + R;
         u32x4 v{0u, 0u, 0u, 0u};
@@ -203,7 +231,6 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
         rpos[nt] = R < nrows ? p0 + t : -1;
         ranc[nt] = p.anc && R < nrows ? p.anc[row0 + t] : 0u;
     }
-    const int t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
     const int lo_max = win_lo(p0 + t_b, p.window), pos_min = p.anc ? p0 - 1 : p0 + t_a;
     __syncthreads();
 
@@ -233,19 +260,45 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
             for (int nt = 0; nt < NT; nt++) st[t][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
         unsigned qo = (unsigned)(ln * Cf::QSTR + 16 * g);              // (opaque: the fragments are read here, not held across steps)
         asm volatile("" : "+v"(qo));
+        if constexpr (KLDS) {
+            // (A wave's LDS operations run in their order: no wait between a unit's writes, its reads and the next one's writes.)
 #pragma unroll
-        for (int d = 0; d < DC; d++) {
-            u32x4 k0[KT], k1[KT];
+            for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int t = 0; t < KT; t++) { k0[t] = e4m3_op<F16>(kr[t][d][0], kr[t][d][1]); k1[t] = e4m3_op<F16>(kr[t][d][2], kr[t][d][3]); }
+                for (int x = 0; x < DC / UD; x++) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const u32x4 q0 = *reinterpret_cast<const u32x4 *>(qs + qo + 16 * nt * Cf::QSTR + 64 * d);
-                const u32x4 q1 = *reinterpret_cast<const u32x4 *>(qs + qo + 16 * nt * Cf::QSTR + 64 * d + 8);
+                    for (int u = 0; u < UD; u++) *reinterpret_cast<u32x4 *>(ks + kw[u]) = kr[t][x * UD + u];
+                    __builtin_amdgcn_wave_barrier();
+                    u32x4 kf[UD];
 #pragma unroll
-                for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k0[t], q0, st[t][nt]);
+                    for (int u = 0; u < UD; u++) kf[u] = *reinterpret_cast<const u32x4 *>(ks + (kfrag ^ (64 * u)));
+                    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k1[t], q1, st[t][nt]);
+                    for (int u = 0; u < UD; u++) {
+                        const u32x4 k0 = e4m3_op<F16>(kf[u][0], kf[u][1]), k1 = e4m3_op<F16>(kf[u][2], kf[u][3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            const uint16_t *q = qs + qo + 16 * nt * Cf::QSTR + 64 * (x * UD + u);
+                            st[t][nt] = mfma16<F16>(k0, *reinterpret_cast<const u32x4 *>(q), st[t][nt]);
+                            st[t][nt] = mfma16<F16>(k1, *reinterpret_cast<const u32x4 *>(q + 8), st[t][nt]);
+                        }
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DC; d++) {
+                u32x4 k0[KT], k1[KT];
+#pragma unroll
+                for (int t = 0; t < KT; t++) { k0[t] = e4m3_op<F16>(kr[t][d][0], kr[t][d][1]); k1[t] = e4m3_op<F16>(kr[t][d][2], kr[t][d][3]); }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const u32x4 q0 = *reinterpret_cast<const u32x4 *>(qs + qo + 16 * nt * Cf::QSTR + 64 * d);
+                    const u32x4 q1 = *reinterpret_cast<const u32x4 *>(qs + qo + 16 * nt * Cf::QSTR + 64 * d + 8);
+#pragma unroll
+                    for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k0[t], q0, st[t][nt]);
+#pragma unroll
+                    for (int t = 0; t < KT; t++) st[t][nt] = mfma16<F16>(k1[t], q1, st[t][nt]);
+                }
             }
         }
         int vf0 = 0, vf1 = 0;
@@ -460,13 +513,19 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     long long keys = max_pos + 1ll;
     if (window > 0) keys = std::min<long long>(keys, (long long)window + T - 1);
     if (pl.prefill) {
-        if (chunk == 0) return pl;
+        if (chunk == 0) { if (getenv("KV8DEC")) { pl.prefill = false; pl.C = 1 << 20; pl.ns = 1; } return pl; }
     } else if (chunk == 0) {
-        const long long units = (long long)B * NKV, want = std::max(1ll, 512 / units);
-        pl.C = (int)std::min<long long>(std::max<long long>((keys / want + 255) / 256 * 256, 256), 1024);
+        // Keys of a split: B * NKV * keys / 700 (1024 for more than 16 rows), in steps, at most 1024. Fewer leave a call to
+        // the prologue of its workgroups, more to its longest one: 16 requests of up to 9K keys at HD 256 took 45.8 us in
+        // 256-key splits, 38.7 in 768 and 53.2 in 2048, one of 9K 15.2 in 256, 13.0 in 128 and 19.2 in 512. Up to three steps
+        // go without splits and their merge (9 instead of 11 us).
+        const long long units = (long long)B * NKV, per = hr <= 16 ? 700 : 1024;
+        pl.C = (int)std::min((units * keys / per + 127) / 128 * 128 + (units * keys < per ? 128 : 0), 1024ll);
+        if (keys <= 384) pl.C = (max_pos / 128 + 1) * 128;
     }
     pl.ns = max_pos / pl.C + 1;
     if (pl.prefill && pl.ns == 1) pl.C = 0;
+    if (getenv("KV8DEC") && pl.prefill) { pl.prefill = false; pl.C = 1 << 20; pl.ns = 1; }
     return pl;
 }
 
