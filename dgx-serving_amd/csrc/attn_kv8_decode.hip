@@ -27,7 +27,6 @@
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 
 namespace dgx {
 
@@ -430,24 +429,35 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
 // added in their order. The weights of the splits are formed once, a thread each (256 at a time). Three dependent reads
 // whatever the number of splits: 64 of them at HD 512 took 15.5 us when every thread walked the maxima and sums itself.
 // Also writes the rows that attend nothing (O = 0, lse = -inf).
+// Where there are many rows, a wave of its own for each (row, q-head, 256 dims) does it without a barrier.
 struct Kv8CombArgs {
     Kv8Problem p;
     Kv8Partials part;
     uint32_t Cm;
 };
 
+// The splits [c0, c0 + n) of a row, and its first element among the partials; false past the last row.
+__device__ __forceinline__ bool comb_row(const Kv8CombArgs &a, int bt, int head, size_t &row, int &c0, int &n) {
+    const Kv8Problem &p = a.p;
+    const int b = bt / p.T, i = bt - b * p.T;
+    int row0, nr;
+    kv8_rows(p, b, row0, nr);
+    if (i >= nr) return false;
+    const int pos = min(p.ctx[b], INT_MAX - i) + i, lo = win_lo(pos, p.window), hi = min(pos, p.max_pos);
+    row = (size_t)(row0 + i) * p.NQ + head;
+    c0 = div_by(lo, a.part.C, a.Cm);
+    n = hi >= lo ? div_by(hi, a.part.C, a.Cm) - c0 + 1 : 0;
+    return true;
+}
+
 __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8CombArgs a) {
     __shared__ __align__(16) float red[8][128];
     __shared__ float wt[256], part_s[2][4];
     const Kv8Problem &p = a.p;
     const int HD = p.c.HD;
-    const int b = (int)blockIdx.x / p.T, i = (int)blockIdx.x - b * p.T, head = blockIdx.y;
-    int row0, nr;
-    kv8_rows(p, b, row0, nr);
-    if (i >= nr) return;
-    const int pos = min(p.ctx[b], INT_MAX - i) + i, lo = win_lo(pos, p.window), hi = min(pos, p.max_pos);
-    const size_t row = (size_t)(row0 + i) * p.NQ + head;
-    const int c0 = div_by(lo, a.part.C, a.Cm), n = hi >= lo ? div_by(hi, a.part.C, a.Cm) - c0 + 1 : 0;
+    size_t row;
+    int c0, n;
+    if (!comb_row(a, (int)blockIdx.x, (int)blockIdx.y, row, c0, n)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, d4 = tid & 31, ph = tid >> 5, dim = (int)blockIdx.z * 128 + 4 * d4;
     const float *pm = a.part.m + row * a.part.ns + c0, *pl = a.part.l + row * a.part.ns + c0;
     const float *pa = a.part.acc + (row * a.part.ns + c0) * HD + dim;
@@ -485,8 +495,62 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8CombArgs a) {
     if (tid == 0 && blockIdx.z == 0 && p.lse) p.lse[row] = L == 0.f ? kNegInf : (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
 
+template <int NP>   // 2 (HD 128): the halves of the wave take the splits in turn
+__global__ void __launch_bounds__(256) kv8_combine_rows_kernel(const Kv8CombArgs a, int units) {
+    const Kv8Problem &p = a.p;
+    const int HD = p.c.HD, lane = threadIdx.x & 63, per = HD > 256 ? HD / 256 : 1;
+    const int u = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
+    if (u >= units) return;
+    const int bt = u / (p.NQ * per), hs = u - bt * p.NQ * per, head = hs / per;
+    size_t row;
+    int c0, n;
+    if (!comb_row(a, bt, head, row, c0, n)) return;
+    const float *pm = a.part.m + row * a.part.ns + c0, *pl = a.part.l + row * a.part.ns + c0;
+    const int ph = NP == 2 ? lane >> 5 : 0, dim = (hs - head * per) * 256 + 4 * (NP == 2 ? lane & 31 : lane);
+    const float *pa = a.part.acc + (row * a.part.ns + c0) * HD + dim;
+    float M = kNegInf;
+    for (int c = lane; c < n; c += 64) M = fmaxf(M, pm[c]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+    for (int b0 = 0; b0 < n; b0 += 64) {
+        const float lc = b0 + lane < n ? pl[b0 + lane] : 0.f;
+        const float w = b0 + lane < n ? kv8_weight(pm[b0 + lane], lc, M) : 0.f;
+        L += lc * w;
+        const int nb = min(64, n - b0);
+        for (int c = 0; c < nb; c += 8 * NP) {                         // eight loads in flight; past the last split: its value, no weight
+            f32x4 t[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++) t[x] = *reinterpret_cast<const f32x4 *>(pa + (size_t)(b0 + min(c + NP * x + ph, nb - 1)) * HD);
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const float wx = __shfl(w, min(c + NP * x + ph, 63));
+                if (c + NP * x + ph < nb) v += t[x] * wx;
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
+    if constexpr (NP == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], 32);
+        if (ph) return;
+    }
+    kv8_store4(p, row * HD + dim, v * (L == 0.f ? 0.f : 1.f / L));
+    if (lane == 0 && hs == head * per && p.lse) p.lse[row] = L == 0.f ? kNegInf : (M + __builtin_amdgcn_logf(L)) * kLn2;
+}
+
 hipError_t launch_kv8_combine(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st) {
     const Kv8CombArgs a{p, part, div_magic(part.C)};
+    const long long units = (long long)p.B * p.T * p.NQ * (p.c.HD > 256 ? p.c.HD / 256 : 1);
+    // 3072 rows in up to 16 splits at HD 256: 12.8 us in workgroups, XX in waves; 128 rows in up to 64 at HD 512 5.0 and XX.
+    if (units >= 1024 && units <= INT_MAX) {
+        const dim3 g4((unsigned)((units + 3) / 4));
+        if (p.c.HD == 128) hipLaunchKernelGGL(kv8_combine_rows_kernel<2>, g4, dim3(256), 0, st, a, (int)units);
+        else hipLaunchKernelGGL(kv8_combine_rows_kernel<1>, g4, dim3(256), 0, st, a, (int)units);
+        return hipGetLastError();
+    }
     const dim3 grid((unsigned)p.B * (unsigned)p.T, (unsigned)p.NQ, (unsigned)p.c.HD / 128);
     hipLaunchKernelGGL(kv8_combine_kernel, grid, dim3(256), 0, st, a);
     return hipGetLastError();
@@ -513,19 +577,20 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     long long keys = max_pos + 1ll;
     if (window > 0) keys = std::min<long long>(keys, (long long)window + T - 1);
     if (pl.prefill) {
-        if (chunk == 0) { if (getenv("KV8DEC")) { pl.prefill = false; pl.C = 1 << 20; pl.ns = 1; } return pl; }
+        if (chunk == 0) return pl;
     } else if (chunk == 0) {
-        // Keys of a split: B * NKV * keys / 700 (1024 for more than 16 rows), in steps, at most 1024. Fewer leave a call to
-        // the prologue of its workgroups, more to its longest one: 16 requests of up to 9K keys at HD 256 took 45.8 us in
-        // 256-key splits, 38.7 in 768 and 53.2 in 2048, one of 9K 15.2 in 256, 13.0 in 128 and 19.2 in 512. Up to three steps
-        // go without splits and their merge (9 instead of 11 us).
-        const long long units = (long long)B * NKV, per = hr <= 16 ? 700 : 1024;
-        pl.C = (int)std::min((units * keys / per + 127) / 128 * 128 + (units * keys < per ? 128 : 0), 1024ll);
+        // Keys of a split, by the call's K and V in heads of 256 dims. Short ones leave a call to the prologues of its
+        // workgroups and the merge, long ones to the longest workgroup. 16 requests of 9K keys x 4 heads (576K) took 42.8 us
+        // in 256-key splits, 37.3 in 512 and 38.7 in 1024; of 32K keys (2M) 113.8 in 512 and 106.7 in 1024; 4 of 9K (144K)
+        // 19.7 in 256, 20.4 in 512 and 30.1 in 1024; one of 9K (36K) 13.0 in 128 and 15.2 in 256. With more than 16 rows the
+        // partials weigh more: 16 trees of 48 rows over 16K keys (1M) 87.7 us in 512 and 72.8 in 1024. Up to three steps go
+        // without splits and their merge (9 instead of 11 us).
+        const long long work = (long long)B * NKV * keys * HD / 256;
+        pl.C = work < 60000 ? 128 : work < 280000 ? 256 : work < (hr > 16 ? 700000 : 1500000) ? 512 : 1024;
         if (keys <= 384) pl.C = (max_pos / 128 + 1) * 128;
     }
     pl.ns = max_pos / pl.C + 1;
     if (pl.prefill && pl.ns == 1) pl.C = 0;
-    if (getenv("KV8DEC") && pl.prefill) { pl.prefill = false; pl.C = 1 << 20; pl.ns = 1; }
     return pl;
 }
 
