@@ -244,14 +244,11 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     for (; s <= s1; s++) {
         const int j0 = SK * s, jw = j0 + 16 * KT * wave;
         const Scales sc = sn;
-        const Own now = cur;
+        const Own now = cur, next = nxt;
         const bool pages_ok = okn;
-        if (s < s1) {                                                  // (these wait together with the K loads of this step)
-            cur = nxt;
-            sn = scales_of(cur);
-            okn = own_ok(cur);
-            nxt = own_ids(min(s + 2, s1));
-        }
+        // (Without a branch around them, and taken over at the end of the step: the scalar loads then wait with the K loads.)
+        const Scales s2 = scales_of(next);
+        const Own n2 = own_ids(min(s + 2, s1));
         f32x4 st[KT][NT];
 #pragma unroll
         for (int t = 0; t < KT; t++)
@@ -303,7 +300,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
         int vf0 = 0, vf1 = 0;
         if (s < s1) {
             vf0 = v_id(min(s + 2, s1), 0); vf1 = v_id(min(s + 2, s1), 1);
-            load_k(s + 1, cur);
+            load_k(s + 1, next);
         }
         const bool full = pages_ok && jw >= j_lo && jw + 16 * KT <= j_hi && jw >= lo_max && jw + 16 * KT - 1 <= pos_min;
 #pragma unroll
@@ -391,6 +388,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
         }
         if (s < s1) { load_v(0, vn0); load_v(1, vn1); }
         vi0 = vn0; vi1 = vn1; vn0 = vf0; vn1 = vf1;
+        cur = next; nxt = n2; sn = s2; okn = own_ok(next);
     }
 
     // Row sums over the waves, in their order; m is the same in all.
