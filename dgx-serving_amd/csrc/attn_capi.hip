@@ -736,7 +736,7 @@ hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const 
         part.l = reinterpret_cast<float *>(static_cast<char *>(ws) + one);
         part.acc = reinterpret_cast<float *>(static_cast<char *>(ws) + 2 * one);
     }
-    const hipError_t e = timed_launch(st, [&] { return pl.prefill ? launch_kv8_prefill(p, part, st) : launch_kv8_decode(p, part, st); });
+    const hipError_t e = timed_launch(st, [&] { return pl.prefill ? launch_kv8_prefill(p, part, st) : launch_kv8_decode(p, part, pl.nt, st); });
     if (e != hipSuccess || pl.ns == 1) return e;
     return launch_kv8_combine(p, part, st);
 }

@@ -105,14 +105,16 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
 hipError_t launch_kv8_append(const void *k, const void *v, int src_dtype, long k_stride, long v_stride, const Kv8 &c,
                              const int *slots, int rows, unsigned *stats, hipStream_t st);
 
-// Split-KV form: single tokens, short runs and trees (any T; rows of a KV head in groups of 16 .. 64).
-hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st);
+// Split-KV form: single tokens, short runs, trees, small prompts (any T; rows of a KV head in groups of 16 nt, nt 1, 2 or 4;
+// at HD 512 1 or 2).
+hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, int nt, hipStream_t st);
 // Prompt form: 64 or 128 rows of a KV head per workgroup, no tree masks.
 hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st);
 hipError_t launch_kv8_combine(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st);
 
-// What a call runs: the form, and the keys of a split (0: one pass that writes O).
-struct Kv8Plan { bool prefill; int C, ns; };
+// What a call runs: the form, the split-KV form's row groups, the keys of a split (0: the prompt form's one pass) and how many
+// splits max_pos reaches (1: the kernel writes O, no workspace).
+struct Kv8Plan { bool prefill; int nt, C, ns; };
 Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, bool tree);
 
 }  // namespace dgx

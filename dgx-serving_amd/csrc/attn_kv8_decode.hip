@@ -1,5 +1,5 @@
-// Split-KV attention over the paged 8-bit cache on gfx950: single tokens, short runs and draft trees, and the merge of key
-// splits.
+// Split-KV attention over the paged 8-bit cache on gfx950: single tokens, short runs, draft trees and prompts that do not fill
+// the chip, and the merge of key splits.
 //
 // A workgroup owns one key chunk of one request and KV head and up to 16 NT of its query rows (token-major: tokens x q-heads
 // of the KV head, so a byte of K or V is read once for the whole group). It walks the chunk in steps of 128 keys at absolute
@@ -36,6 +36,7 @@ struct Kv8DecArgs {
     int C;                            // keys of a chunk
     uint32_t Cm;                      // div_magic(C)
     int nrg;                          // row groups of a KV head
+    int spread;                       // > 0: (chunk, KV head) units, which the row groups take in turn
     int direct;                       // one chunk holds every key: O and lse are written here
     float sl2;                        // scale * log2(e)
 };
@@ -102,8 +103,11 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     extern __shared__ __align__(16) unsigned char smem[];
     const Kv8Problem &p = a.p;
     const Kv8 &kc = p.c;
-    // Workgroups of one (chunk, KV head) and different row groups read the same keys: 8 apart, on one XCD.
-    const int unit = (int)(blockIdx.x / (8 * a.nrg)) * 8 + (int)(blockIdx.x & 7), rg = a.nrg - 1 - (int)(blockIdx.x >> 3) % a.nrg;
+    // Workgroups of one (chunk, KV head) and different row groups read the same keys: 8 apart, on one XCD, if there are enough
+    // of them for all XCDs.
+    int unit, rg;
+    if (a.spread) { rg = a.nrg - 1 - (int)blockIdx.x / a.spread; unit = (int)blockIdx.x % a.spread; }
+    else { unit = (int)(blockIdx.x / (8 * a.nrg)) * 8 + (int)(blockIdx.x & 7); rg = a.nrg - 1 - (int)(blockIdx.x >> 3) % a.nrg; }
     int seq, c, lo, hi;
     if (!kv8_find(p, a.C, a.Cm, a.direct, unit / kc.NKV, seq, c, lo, hi)) return;
     seq = __builtin_amdgcn_readfirstlane(seq); c = __builtin_amdgcn_readfirstlane(c);
@@ -569,36 +573,54 @@ template <int HD, int NT> static hipError_t launch_dec_n(const Kv8DecArgs &a, di
 }
 
 Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, bool tree) {
-    (void)rows;
-    const long long hr = (long long)T * (NQ / NKV);                    // rows of a KV head and request
-    Kv8Plan pl{!tree && hr > 64, chunk, 1};
+    const long long G = NQ / NKV, hr = T * G;                          // rows of a KV head and request
     long long keys = max_pos + 1ll;
     if (window > 0) keys = std::min<long long>(keys, (long long)window + T - 1);
-    if (pl.prefill) {
-        if (chunk == 0) return pl;
-    } else if (chunk == 0) {
+    const int whole = (max_pos / 128 + 1) * 128;                       // a split that holds every key
+    Kv8Plan pl{false, 0, chunk, 1};
+    if (tree || hr <= 64) {
+        pl.nt = hr <= 16 ? 1 : hr <= 32 || HD == 512 ? 2 : 4;
         // Keys of a split, by the call's K and V in heads of 256 dims. Short ones leave a call to the prologues of its
         // workgroups and the merge, long ones to the longest workgroup. 16 requests of 9K keys x 4 heads (576K) took 42.8 us
         // in 256-key splits, 37.3 in 512 and 38.7 in 1024; of 32K keys (2M) 113.8 in 512 and 106.7 in 1024; 4 of 9K (144K)
         // 19.7 in 256, 20.4 in 512 and 30.1 in 1024; one of 9K (36K) 13.0 in 128 and 15.2 in 256. With more than 16 rows the
-        // partials weigh more: 16 trees of 48 rows over 16K keys (1M) 87.7 us in 512 and 72.8 in 1024. Up to three steps go
-        // without splits and their merge (9 instead of 11 us).
+        // partials weigh more: 16 trees of 48 rows over 16K keys (1M) 87.7 us in 512 and 72.8 in 1024. Up to four steps go
+        // without splits and their merge (9.5 us for 512 keys of 4 heads of 128, 10.4 in two splits).
         const long long work = (long long)B * NKV * keys * HD / 256;
-        pl.C = work < 60000 ? 128 : work < 280000 ? 256 : work < (hr > 16 ? 700000 : 1500000) ? 512 : 1024;
-        if (keys <= 384) pl.C = (max_pos / 128 + 1) * 128;
+        if (chunk == 0) pl.C = work < 60000 ? 128 : work < 280000 ? 256 : work < (hr > 16 ? 700000 : 1500000) ? 512 : 1024;
+        if (chunk == 0 && keys <= 512) pl.C = whole;
+    } else {
+        // Tiles of 64 rows. Where they do not fill the chip the split-KV form takes a prompt too: it walks 128 keys a step,
+        // and its row groups can be smaller and its keys split.
+        const long long n64 = std::min((long long)B * ((hr + 63) / 64), (long long)rows * G / 64 + B) * NKV;
+        pl.prefill = n64 >= 400;
+        if (!pl.prefill) {
+            // 200 x 16 q-heads over 8 without a prefix: groups of 16 rows 9.5 us, 32 12.2, 64 16.9, the tile kernel 11.4;
+            // 1000 behind 1000: 72, 53, 64 and 60; 512 behind 4096: 64 rows in 1536-key splits 74, in 1024 87, no split of 16
+            // rows 93, the tile kernel in 1024-key splits 85. Fewer workgroups at HD 512: 500 x 16 over 1 behind 4000 117
+            // us unsplit, 138 in 1536; 100 behind 4000 41 in 1024, 52 in 512.
+            const long long n = HD == 512 ? n64 * 2 : n64, want = HD == 512 ? 200 : 450;
+            pl.nt = HD == 512 ? 2 : 4;
+            if (chunk == 0 && keys <= 1280) pl.nt = 1, pl.C = whole;
+            else if (chunk == 0 && keys <= 2304 && n64 >= 128) pl.nt = 2, pl.C = whole;
+            else if (chunk == 0) {
+                const long long splits = std::max(1ll, (want + n / 2) / n);
+                pl.C = splits == 1 ? whole : (int)std::min(2048ll, std::max(512ll, (keys / splits + 127) / 128 * 128));
+            }
+        } else if (chunk == 0) return pl;
     }
     pl.ns = max_pos / pl.C + 1;
     if (pl.prefill && pl.ns == 1) pl.C = 0;
     return pl;
 }
 
-hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st) {
+hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, int nt, hipStream_t st) {
     const int G = p.NQ / p.c.NKV, rows = (int)std::min<long long>((long long)p.T * G, INT_MAX);
-    const int nt = rows <= 16 ? 1 : rows <= 32 || p.c.HD == 512 ? 2 : 4;
-    Kv8DecArgs a{p, part, part.C, div_magic(part.C), (rows + 16 * nt - 1) / (16 * nt), part.ns == 1, p.scale * kLog2e};
+    Kv8DecArgs a{p, part, part.C, div_magic(part.C), (rows + 16 * nt - 1) / (16 * nt), 0, part.ns == 1, p.scale * kLog2e};
     long long per = p.max_pos / part.C + 1;
     if (p.window > 0) per = std::min<long long>(per, ((long long)p.window + p.T - 2) / part.C + 2);
-    const long long units = (per * p.B * p.c.NKV + 7) / 8 * 8, wgs = units * a.nrg;
+    const long long raw = per * p.B * p.c.NKV, units = a.nrg == 1 || raw < 64 ? raw : (raw + 7) / 8 * 8, wgs = units * a.nrg;
+    if (a.nrg == 1 || raw < 64) a.spread = (int)raw;
     if (wgs > INT_MAX) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)wgs);
     switch (p.c.HD) {

@@ -23,7 +23,6 @@
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 
 namespace dgx {
 
@@ -288,25 +287,20 @@ __global__ void __launch_bounds__(Cf::NW * 64, Cf::OCC) kv8_prefill_kernel(const
             unsigned ka = kaddr + (unsigned)(s & 1) * Cf::STAGE + 32 * x * HD;
             unsigned va = (vaddr + (((unsigned)(2 * (kg * NSUB + x) + (g >> 1)) ^ (unsigned)vf(ln)) << 4)) + (unsigned)(s & 1) * Cf::STAGE;
             asm volatile("" : "+v"(ka), "+v"(va));
-            u32x4 kw[2][2];
-            auto read_k = [&](int d) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) kw[d & 1][t] = *lds_at<u32x4>((ka ^ (64 * d)) + 4 * t * HD);
-            };
+            // Fragment 2 d + t is read while the one before it is multiplied (one, not more: registers).
+            u32x4 kw[2];
+            auto read_k = [&](int i) { kw[i & 1] = *lds_at<u32x4>((ka ^ (64 * (i >> 1))) + 4 * (i & 1) * HD); };
             read_k(0);
 #pragma unroll
-            for (int d = 0; d < DC; d++) {
-                if (d + 1 < DC) read_k(d + 1);
+            for (int i = 0; i < 2 * DC; i++) {
+                if (i + 1 < 2 * DC) read_k(i + 1);
                 __builtin_amdgcn_sched_barrier(0);
-                const u32x4 (&w)[2] = kw[d & 1];
+                const int d = i >> 1, t = i & 1;
+                const u32x4 k0 = e4m3_op<F16>(kw[t][0], kw[t][1]), k1 = e4m3_op<F16>(kw[t][2], kw[t][3]);
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const u32x4 k0 = e4m3_op<F16>(w[t][0], w[t][1]), k1 = e4m3_op<F16>(w[t][2], w[t][3]);
+                for (int rb = 0; rb < RB; rb++) st[t][rb] = mfma16<F16>(k0, qop[rb][2 * d], st[t][rb]);
 #pragma unroll
-                    for (int rb = 0; rb < RB; rb++) st[t][rb] = mfma16<F16>(k0, qop[rb][2 * d], st[t][rb]);
-#pragma unroll
-                    for (int rb = 0; rb < RB; rb++) st[t][rb] = mfma16<F16>(k1, qop[rb][2 * d + 1], st[t][rb]);
-                }
+                for (int rb = 0; rb < RB; rb++) st[t][rb] = mfma16<F16>(k1, qop[rb][2 * d + 1], st[t][rb]);
             }
             const bool up = g >= 2, ok = up ? sc.ok[x][1] : sc.ok[x][0];   // the lane's 8 keys are in piece g / 2 of the sub-step's
             // (the factor stays above zero: a hidden score is -inf before it is multiplied)
@@ -485,19 +479,15 @@ hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, hipS
         if (p.window > 0) per = std::min<long long>(per, ((long long)p.window + p.T - 2) / part.C + 2);
         a.ns = (int)std::max(2ll, per);
     }
-    const int var = getenv("KV8V") ? atoi(getenv("KV8V")) : 0;
+    // Tiles of 128 rows where there are two rounds of them for the 512 workgroups that run at once (one, under a window: its
+    // tiles are equally long), else of 64. HD 256, TFLOP/s of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400
+    // tiles of 128) 853 | 732, 4096 behind a window of 1024, 16 over 8 (512 tiles) 666 | 598, causal 4000 of those (500) 604 | 776.
+    const long long rows = std::min((long long)p.B * p.T, (long long)p.rows) * G * p.c.NKV * a.ns;
+    const bool wide = rows >= 128 * (p.window > 0 && p.window < p.max_pos ? 500 : 960);
     switch (p.c.HD) {
-    case 128: 
-        if (var == 1) return launch_pre<128, Kv8PrefCfg<128, 1, 2, 2, 1, 3>>(a, st);
-        if (var == 2) return launch_pre<128, Kv8PrefCfg<128, 2, 4, 1, 2, 2>>(a, st);
-        return launch_pre<128, Kv8PrefCfg<128, 2, 2, 2, 1, 3>>(a, st);
-    case 256:
-        if (var == 1) return launch_pre<256, Kv8PrefCfg<256, 1, 2, 2, 1, 2>>(a, st);
-        if (var == 2) return launch_pre<256, Kv8PrefCfg<256, 2, 4, 1, 2, 2>>(a, st);
-        return launch_pre<256, Kv8PrefCfg<256, 2, 2, 2, 1, 2>>(a, st);
-    case 512: 
-        if (var == 1) return launch_pre<512, Kv8PrefCfg<512, 1, 4, 1, 2, 1>>(a, st);
-        if (var == 2) return launch_pre<512, Kv8PrefCfg<512, 1, 2, 2, 1, 1>>(a, st);
+    case 128: return wide ? launch_pre<128, Kv8PrefCfg<128, 2, 4, 1, 2, 2>>(a, st) : launch_pre<128, Kv8PrefCfg<128, 2, 2, 2, 1, 3>>(a, st);
+    case 256: return wide ? launch_pre<256, Kv8PrefCfg<256, 2, 4, 1, 2, 2>>(a, st) : launch_pre<256, Kv8PrefCfg<256, 2, 2, 2, 1, 2>>(a, st);
+    case 512:                                                          // (64 rows in 8 waves: 4 of 1500 x 16 q-heads 299 us, in 4 waves 333, 32 rows 444)
         return launch_pre<512, Kv8PrefCfg<512, 1, 4, 2, 1, 2>>(a, st);
     default: return hipErrorInvalidValue;
     }
