@@ -351,6 +351,8 @@ bool kv8_sizes_ok(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, 
            max_pos < kKv8MaxPos && chunk >= 0 && chunk <= kKv8MaxChunk && chunk % 64 == 0 && (long long)B * T <= INT_MAX &&
            T <= kKv8MaxPos && (long long)T * (NQ / NKV) <= INT_MAX / 2;
 }
+// Partials of a call past this are refused (2^40 of them are 128 TiB): no product below then passes 64 bits.
+bool kv8_partials_ok(int rows, int NQ, int ns) { return (long long)rows * NQ <= (1ll << 40) / ns; }
 // Bytes of the partials of a call: m and l [rows * NQ * ns], each rounded up to 256 bytes, then acc.
 size_t kv8_bytes(size_t partials, int HD) { return 2 * ((partials * 4 + 255) / 256 * 256) + partials * (size_t)HD * 4; }
 
@@ -710,6 +712,7 @@ size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, i
     if (!kv8_sizes_ok(B, T, rows, NQ, NKV, HD, max_pos, chunk)) return (size_t)-1;
     if (B == 0 || T == 0 || rows == 0) return 0;
     const Kv8Plan pl = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window < 0 ? 0 : window, tree != 0);
+    if (pl.ns > 1 && !kv8_partials_ok(rows, NQ, pl.ns)) return (size_t)-1;
     return pl.ns > 1 ? kv8_bytes((size_t)rows * NQ * pl.ns, HD) : 0;
 }
 
@@ -731,7 +734,7 @@ hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const 
     Kv8Partials part{nullptr, nullptr, nullptr, pl.ns, pl.C};
     if (pl.ns > 1) {
         const size_t n = (size_t)rows * NQ * pl.ns, one = (n * 4 + 255) / 256 * 256;
-        if (!ws || ws_bytes < kv8_bytes(n, c.HD)) return hipErrorInvalidValue;
+        if (!ws || !kv8_partials_ok(rows, NQ, pl.ns) || ws_bytes < kv8_bytes(n, c.HD)) return hipErrorInvalidValue;
         part.m = static_cast<float *>(ws);
         part.l = reinterpret_cast<float *>(static_cast<char *>(ws) + one);
         part.acc = reinterpret_cast<float *>(static_cast<char *>(ws) + 2 * one);

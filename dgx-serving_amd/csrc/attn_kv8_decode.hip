@@ -119,7 +119,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     const int rho0 = rg * Cf::RR, nrows = min(nr * G - rho0, Cf::RR);
     if (nrows <= 0) return;
     // Keys of the chunk that some row of this group attends.
-    const int p0 = scalar_load(p.ctx + seq), t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
+    const int p0 = min(scalar_load(p.ctx + seq), INT_MAX - nr), t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
     const int j_lo = max(c * a.C, win_lo(p0 + t_a, p.window)), j_hi = min(min(hi, p0 + t_b + 1) - c * a.C, a.C) + c * a.C;
     if (j_lo >= j_hi && !a.direct) return;
 

@@ -32,7 +32,7 @@ def attn(c=None, **kw):
                                 dict(B=-1), dict(T=-1), dict(rows=-1), dict(NQ=0), dict(NQ=23), dict(max_pos=-1), dict(max_pos=1 << 30),
                                 dict(chunk=-64), dict(chunk=32), dict(chunk=100), dict(chunk=(1 << 20) + 64), dict(stride=9),
                                 dict(Q=PTR + 8), dict(O=PTR + 2), dict(ws=PTR + 4), dict(cu=None, rows=3), dict(anc=PTR, T=33, rows=66),
-                                dict(ws=None, chunk=64), dict(ws_bytes=100, chunk=64), dict(B=1 << 20, T=1 << 20), dict(NQ=4 * 16384)])
+                                dict(ws=None, chunk=64), dict(ws_bytes=100, chunk=64), dict(B=1, T=1 << 29, rows=1 << 29, NQ=4, max_pos=(1 << 30) - 1, chunk=64, stride=1 << 24), dict(B=1 << 20, T=1 << 20), dict(NQ=4 * 16384)])
 def test_attention_refuses(kw):
     assert attn(**kw) == INVALID
 

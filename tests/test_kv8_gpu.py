@@ -213,7 +213,7 @@ HEADS = {"q6": (24, 4, 256), "g2": (4, 2, 256), "g16": (16, 1, 512), "s4": (8, 2
 
 
 def attn_case(seed, heads, page, io, ctx, add, window=0, tree=False, chunk=0, out=None, spread=2, uniform=False, scale=0.0, hurt=None,
-              max_pos=None, T=None, garbage=True, ws=None):
+              max_pos=None, T=None):
     """One call against the 64-bit form, with NaN codes in every token that is nobody's."""
     NQ, NKV, HD = HEADS[heads]
     rng = np.random.default_rng(seed)
@@ -222,8 +222,7 @@ def attn_case(seed, heads, page, io, ctx, add, window=0, tree=False, chunk=0, ou
     P = int(sum(-(-int(max(n, 0)) // page) for n in lens)) + 2
     table = R.tables(rng, np.maximum(lens, 0), page, P, int(-(-max(lens.max(), 1) // page)) + 1)
     K, V, Ks, Vs = R.make_cache(rng, P, page, NKV, HD, spread)
-    if garbage:
-        R.blank_tail(K, V, table, np.maximum(lens, 0), page)
+    R.blank_tail(K, V, table, np.maximum(lens, 0), page)
     if hurt:
         hurt(K, V, Ks, Vs, table)
     cu = np.concatenate([[0], np.cumsum(add)])
@@ -287,10 +286,72 @@ def test_prompts(heads, io, page, add, window):
         attn_case(8, heads, page, io, [190] * len(add), add, chunk=64, out="fp32")
 
 
-def test_prompts_of_the_wide_tile():
-    """Enough 128-row tiles for the two-block form, at HD 256 and 128."""
-    attn_case(9, "g2", 64, "bf16", [0, 30] * 9, [129, 200] * 9)
-    attn_case(10, "s4", 16, "f16", [5, 0, 64] * 11, [90, 33, 64] * 11, window=70)
+# Sizes from which a call takes each tile (see kv8_choose): (heads, page, ctx, add, window), checked against the rule.
+FORMS = {
+    "128 rows, HD 256": ("q6", 64, [0, 30, 500], [800, 1111, 1500], 0),
+    "128 rows, HD 256, window": ("g2x8", 16, [40], [4001], 300),
+    "128 rows, HD 128": ("s4", 32, [5, 0, 64] * 9, [1200, 400, 333] * 9, 0),
+    "64 rows, HD 256": ("g2x8", 64, [7], [1800], 0),
+    "64 rows, HD 128, window": ("s4", 16, [100, 0], [3100, 3500], 500),
+    "64 rows, HD 512": ("g16", 64, [3, 0, 77], [600, 601, 512], 0),
+    "split, 64-row groups": ("q6", 64, [3000, 2500], [64, 33], 0),
+    "split, 32-row groups, HD 512": ("g16", 16, [3000, 1], [100, 65], 0),
+    "32-row groups, unsplit": ("g2x8", 32, [900], [1000], 0),
+    "16-row groups, unsplit": ("q6", 16, [0, 100, 3], [150, 20, 1], 0),
+}
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_every_form_of_prompts(form):
+    """Rows of the last tiles, of tile and request borders and some between, of larger calls: each against its 64-bit value."""
+    heads, page, ctx, add, window = FORMS[form]
+    NQ, NKV, HD = dict(HEADS, g2x8=(16, 8, 256))[heads]
+    rng = np.random.default_rng(len(form))
+    ctx, add = np.array(ctx), np.array(add)
+    lens = ctx + add
+    P = int((-(-lens // page)).sum()) + 1
+    table = R.tables(rng, lens, page, P)
+    K, V, Ks, Vs = R.make_cache(rng, P, page, NKV, HD)
+    R.blank_tail(K, V, table, lens, page)
+    cu = np.concatenate([[0], np.cumsum(add)])
+    rows = int(cu[-1])
+    Q = torch.from_numpy(rng.standard_normal((rows, NQ, HD))).to(torch.bfloat16)
+    O, lse = torch.full((rows + 1, NQ, HD), 77.0, dtype=torch.bfloat16, device="cuda"), torch.empty(rows, NQ, device="cuda")
+    A.attn_kv8(Q.cuda(), R.to_cache(A, K, V, Ks, Vs), i32(table), i32(ctx), O[:rows], int(add.max()), int(lens.max()) - 1, cu=i32(cu),
+               window=window, lse=lse)
+    torch.cuda.synchronize()
+    assert bool((O[rows] == 77).all()) and not bool((O[:rows] == 77).all(-1).any()) and bool(torch.isfinite(O.float()).all())
+    G = NQ // NKV
+    edges = {t * 64 // G + d for t in range(0, rows * G // 64 + 1, max(1, rows * G // 64 // 6)) for d in (-1, 0)}
+    some = sorted({int(r) for b in range(len(add)) for r in (cu[b], cu[b + 1] - 1)} | {int(r) for r in rng.integers(0, rows, 12)} |
+                  {r for r in edges if 0 <= r < rows})
+    seq = np.searchsorted(cu, some, side="right") - 1
+    for r, b in zip(some, seq):
+        one = R.attention(Q[r:r + 1].double().numpy(), K, V, Ks, Vs, table[b:b + 1], [int(ctx[b] + r - cu[b])], np.array([0, 1]), window=window)
+        R.check(O[r:r + 1], lse[r:r + 1], one, f"{form}, row {r}")
+
+
+def test_prompts_of_many_requests():
+    """More requests than lanes, some empty, in every form: the order of tiles and items."""
+    rng = np.random.default_rng(9)
+    attn_case(9, "s4", 16, "f16", rng.integers(0, 90, 70), rng.integers(0, 4, 70))
+    attn_case(10, "g2", 64, "bf16", [0, 30] * 9, [129, 200] * 9)
+    add = rng.integers(0, 60, 130)
+    add[3] = 80
+    attn_case(11, "g1", 16, "bf16", rng.integers(0, 90, 130), add, window=70)
+    attn_case(12, "s4", 16, "f16", [5, 0, 64] * 11, [90, 33, 64] * 11, window=70)
+
+
+@pytest.mark.parametrize("heads,B,T", [("q6", 8, 8), ("s4", 30, 5), ("g16", 9, 4)])
+def test_merge_of_many_rows(heads, B, T):
+    """Enough rows for the merge by waves; requests without keys in some splits, and without rows."""
+    rng = np.random.default_rng(B)
+    ctx, add = rng.integers(0, 400, B), rng.integers(0, T + 1, B)
+    add[0] = T
+    assert B * T * HEADS[heads][0] * max(1, HEADS[heads][2] // 256) >= 1024  # a unit is a row and head of up to 256 dims
+    attn_case(13, heads, 32, "f16", ctx, add, chunk=64)
+    attn_case(14, heads, 16, "bf16", ctx, add, chunk=128, window=90, out="fp32")
+    attn_case(15, heads, 16, "bf16", ctx, add, chunk=64, tree=True)
 
 
 @pytest.mark.parametrize("io,out", [("f16", "f16"), ("f16", "bf16"), ("f16", "fp32"), ("bf16", "f16"), ("bf16", "fp32")])
@@ -423,11 +484,6 @@ def test_cache_past_4_gib():
 
 
 # ---------------------------------------------------------------- together
-def steps(page, NQ, NKV, HD, rng, B, P, n_steps, first):
-    for step in range(n_steps):
-        yield np.array(first if step == 0 else [1] * B)
-
-
 def test_a_serving_run_of_the_three_together():
     """Prompts, then single tokens, then a draft: tables, append and attention of each step from the lengths alone, and pages
     given back and taken again."""
@@ -540,6 +596,107 @@ def test_a_captured_step_replays_on_new_lengths():
                 kv = torch.randn(2, sum(big), NKV, HD, device="cuda", generator=g)
                 A.kv8_append(kv[0], kv[1], s.cache, slots)
                 s.ctx.add_(i32(big))
+
+
+def test_captured_prompts():
+    """A prompt of the tile kernel at HD 512 (dynamic LDS past 64 KB) and a split one, each captured and replayed on new lengths."""
+    rng = np.random.default_rng(21)
+    for heads, T, ctx, mp in (("g16", 1700, 0, 1699), ("q6", 64, 2000, 3000)):
+        NQ, NKV, HD = HEADS[heads]
+        K, V, Ks, Vs = R.make_cache(rng, mp // 64 + 3, 64, NKV, HD)
+        cache = R.to_cache(A, K, V, Ks, Vs)
+        table = i32(rng.permutation(mp // 64 + 3)[None])
+        Q = torch.randn(T, NQ, HD, device="cuda").half()
+        c, cu = i32([ctx]), i32([0, T])
+        ws = torch.empty(A.attn_kv8_workspace(1, T, T, NQ, NKV, HD, mp), dtype=torch.uint8, device="cuda")
+        O, E = torch.zeros_like(Q), torch.zeros_like(Q)
+        A.attn_kv8(Q, cache, table, c, E, T, mp, cu=cu, ws=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            A.attn_kv8(Q, cache, table, c, O, T, mp, cu=cu, ws=ws)
+        for n in (T, T - 5, 1, T // 2):
+            cu.copy_(i32([0, n]))
+            c.copy_(i32([ctx + T - n]))
+            O.fill_(2.0), E.fill_(2.0)
+            g.replay()
+            A.attn_kv8(Q, cache, table, c, E, T, mp, cu=cu, ws=torch.empty_like(ws))
+            torch.cuda.synchronize()
+            assert torch.equal(O, E), (heads, n)
+
+
+def test_tables_with_strided_rows():
+    """A table whose rows lie further apart than their columns, in all three operators."""
+    NQ, NKV, HD = HEADS["s4"]
+    rng = np.random.default_rng(22)
+    K, V, Ks, Vs = R.make_cache(rng, 20, 16, NKV, HD)
+    cache = R.to_cache(A, K, V, Ks, Vs)
+    big = i32(np.full((3, 40), -9))
+    table = big[:, 4:11]
+    ctx, add = np.array([0, 0, 0]), np.array([40, 0, 100])
+    cu, slots, n, status = i32([0] * 4), i32([0] * 140), i32([20]), i32([0])
+    free = rng.permutation(20)
+    A.kv8_plan(i32(ctx), i32(add), 16, table, i32(free), n, n, cu, slots, status)
+    want = ref_plan(ctx, add, 16, np.full((3, 7), -9), free, 20, 140)
+    assert int(status[0]) == 0 and np.array_equal(table.cpu().numpy(), want[1]) and np.array_equal(slots.cpu().numpy(), want[3])
+    assert bool((big[:, :4] == -9).all()) and bool((big[:, 11:] == -9).all())
+    kt, k = values(rng, 140, NKV, HD, "bf16")
+    A.kv8_append(kt, kt, cache, slots)
+    R.append(K, V, Ks, Vs, k, k, want[3])
+    for T, rows_of in ((100, [40, 0, 100]), (1, [1, 0, 1])):
+        q = np.array(rows_of)
+        c = ctx + add - q
+        off = np.concatenate([[0], np.cumsum(q)])
+        Q = torch.randn(int(off[-1]), NQ, HD, device="cuda").half()
+        O = torch.empty_like(Q)
+        A.attn_kv8(Q, cache, table, i32(c), O, T, 99, cu=i32(off))
+        R.check(O, None, R.attention(Q.double().cpu().numpy(), K, V, Ks, Vs, want[1], c, off), str(T))
+
+
+def test_what_the_binding_refuses_on_the_gpu():
+    NQ, NKV, HD = HEADS["s4"]
+    cache = A.KV8Cache.empty(4, 16, NKV, HD)
+    Q = torch.zeros(2, NQ, HD, device="cuda").half()
+    t, c = i32([[0], [1]]), i32([3, 4])
+    good = dict(Q=Q, cache=cache, table=t, ctx=c, O=torch.empty_like(Q), T=1, max_pos=10)
+    A.attn_kv8(**good)
+    for bad in (dict(max_pos=16), dict(O=torch.empty_like(Q)[:1]), dict(Q=Q.float()), dict(Q=Q.transpose(0, 1).contiguous().transpose(0, 1)),
+                dict(table=t.long()), dict(table=t.expand(2, 3)), dict(ctx=c.float()), dict(cu=i32([0, 2])), dict(anc=i32([1])),
+                dict(lse=torch.empty(2, NQ, device="cuda").half()), dict(ws=torch.empty(8, device="cuda")), dict(cu=torch.zeros(3, dtype=torch.int32))):
+        with pytest.raises((ValueError, A.HipError)):
+            A.attn_kv8(**dict(good, **bad))
+    k = torch.zeros(3, NKV, HD, device="cuda")
+    s = i32([0, 1, 2])
+    A.kv8_append(k, k, cache, s)
+    for bad in ((k.double(), k.double(), s), (k, k.half(), s), (k[:2], k, s), (k, k, s.long()), (k[..., ::2], k, s),
+                (torch.zeros(3, NKV, HD + 1, device="cuda")[..., 1:], k, s), (k[:1].expand(3, NKV, HD), k, s)):
+        with pytest.raises((ValueError, A.HipError)):
+            A.kv8_append(bad[0], bad[1], cache, bad[2])
+
+
+def test_statistics_of_the_append():
+    """G4_KV_STATS=1 counts what is not finite and the largest stored magnitudes, as the other stores do."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = ["dgx-serving_amd", "tests"]
+import torch, dgx_attn as A
+c = A.KV8Cache.empty(3, 16, 2, 128)
+k, v = torch.ones(20, 2, 128, device="cuda") * 3.3, torch.ones(20, 2, 128, device="cuda")
+k[4, 1, 9] = -100.3; k[2, 0, 0] = float("nan"); v[3, 1, 5] = float("inf"); v[17, 0, 7] = float("-inf"); v[19, 1, 127] = 7.7
+A.kv8_append(k, v, c, torch.arange(20, dtype=torch.int32, device="cuda"))
+torch.cuda.synchronize()
+s = A.kv_stats()
+f = lambda u: torch.tensor([u], dtype=torch.int64).to(torch.int32).view(torch.float32).item()
+print(s[0], s[1], f(s[2]), f(s[3]))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, G4_KV_STATS="1"), cwd=root, capture_output=True, text=True, timeout=110)
+    assert out.returncode == 0, out.stderr
+    # 100.3 under 2^-2 is 401.2, nearest code 416: 104. 7.7 under 2^-5 (7.7 <= 448 / 32) is 246.4, nearest 240 (step 16): 7.5
+    assert out.stdout.split() == ["1", "2", "104.0", "7.5"], out.stdout
 
 
 def test_streams_with_their_own_workspaces():
