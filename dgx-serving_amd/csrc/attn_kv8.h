@@ -6,7 +6,7 @@
 //   * x / 2^e is exact, so a stored value is off by one rounding to e4m3 and by nothing else,
 //   * a page whose scale grows keeps the bits of its codes but for those that leave the normal range,
 //   * the attention kernels fold the K scale into the factor that the scores are multiplied by anyway and the V scale into
-//     the exponent of the probabilities (see weight2 below): neither costs an operation per element.
+//     the exponent of the probabilities (P = 2^(s + e - m) multiplies the bare codes): neither costs an operation per element.
 // Layout, chosen for the matrix operands (16 bytes per lane straight from memory, no transpose in any kernel):
 //   K  [pages][NKV][page][HD]      V  [pages][NKV][HD][page]      Ks, Vs  [pages][NKV]
 #pragma once
@@ -31,7 +31,9 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
     return min(max(e, kv8_emin), kv8_emax);
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
-__device__ __forceinline__ int exp_of(float scale) { return (int)((__float_as_uint(scale) >> 23) & 255u) - 127; }
+// Exponent of a scale, at most 126: the scale of a page that holds no token yet may be anything, its keys weigh 0, and 0 times
+// 2^-exponent has to stay 0.
+__device__ __forceinline__ int exp_of(float scale) { return min((int)((__float_as_uint(scale) >> 23) & 255u), 253) - 127; }
 
 // Two e4m3 codes (bytes 2 * HI, 2 * HI + 1 of w) as a packed pair of 16-bit MFMA operands; exact in either format.
 template <bool F16, bool HI> __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
@@ -75,8 +77,8 @@ __device__ __forceinline__ void kv8_rows(const Kv8Problem &p, int b, int &r0, in
     }
 }
 
-// Partials of a split call: index (r * NQ + head) * ns + split; acc[HD], reference exponent m and sum l (see
-// Kv8Partials::weight in the kernels): the row's output is sum acc 2^(m - M) / sum l 2^(m - M).
+// Partials of a split call: index (r * NQ + head) * ns + split; acc[HD], reference exponent m and sum l: the row's output is
+// sum acc 2^(m - M) / sum l 2^(m - M) over the splits, M the largest m.
 struct Kv8Partials {
     float *m, *l, *acc;
     int ns, C;                        // splits of a row at most, keys of a split (0: none, the kernel writes O itself)
@@ -98,6 +100,9 @@ __device__ __forceinline__ void kv8_store4(const Kv8Problem &p, size_t at, const
 // Merge weight of a partial state (m, l) under the common reference M >= m. A state that saw no key has m = -inf and
 // l = 0; one whose only keys were NaN has m = -inf and l = NaN, which must reach the result.
 __device__ __forceinline__ float kv8_weight(float m, float l, float M) { return m == kNegInf ? l * 0.f : fast_exp2(m - M); }
+
+// A launch holds less than 2^32 threads.
+inline bool kv8_grid_ok(long long wgs, int threads) { return wgs <= 0x7fffffff && wgs * threads <= 0xffffffffll; }
 
 hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *table, long table_stride, int cols,
                            const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots, int rows,

@@ -8,7 +8,7 @@
 //   * K and V go from memory to the matrix units through registers alone, and every code is loaded and converted to 16 bits
 //     (exactly) once per workgroup: half the accumulators per wave would be twice the conversions, and the other way round;
 //   * a wave holds 16 rows x HD / NW dims of the output (16 registers at HD 256 instead of the 64 of a wave that walks its
-//     own keys), which leaves registers for 3 to 4 waves per SIMD, and there is no merge of waves at the end;
+//     own keys), which leaves registers for 2 to 4 waves per SIMD (OCC below), and there is no merge of waves at the end;
 //   * the price is two barriers a step: for the row maxima, and for the probabilities.
 // S^T = K Q^T on 16x16x32: a lane's 16-byte load is 16 dims of one key, two operands. O^T += V^T P^T: V pages hold
 // [dim][token], so a lane's 16-byte load is 16 consecutive tokens of one dim, and its P operand is 16 neighbouring
@@ -436,15 +436,26 @@ struct Kv8CombArgs {
     Kv8Problem p;
     Kv8Partials part;
     uint32_t Cm;
+    int by_row;                       // items are rows of the buffers, not the T rows that each request has at most
 };
 
-// The splits [c0, c0 + n) of a row, and its first element among the partials; false past the last row.
+// The splits [c0, c0 + n) of item bt's row, and the row's first element among the partials; false past the last row. All lanes
+// of a wave ask for the same item.
 __device__ __forceinline__ bool comb_row(const Kv8CombArgs &a, int bt, int head, size_t &row, int &c0, int &n) {
     const Kv8Problem &p = a.p;
-    const int b = bt / p.T, i = bt - b * p.T;
-    int row0, nr;
-    kv8_rows(p, b, row0, nr);
-    if (i >= nr) return false;
+    int b, i, row0, nr;
+    if (a.by_row) {                                                    // the request: as many begin at or before the row
+        const int lane = threadIdx.x & 63;
+        b = -1;
+        for (int s0 = 0; s0 < p.B; s0 += 64) b += __builtin_popcountll(__ballot(s0 + lane < p.B && p.cu[min(s0 + lane, p.B)] <= bt));
+        if (b < 0) return false;
+        kv8_rows(p, b, row0, nr);
+        i = bt - row0;
+    } else {
+        b = bt / p.T; i = bt - b * p.T;
+        kv8_rows(p, b, row0, nr);
+    }
+    if ((unsigned)i >= (unsigned)nr) return false;
     const int pos = min(p.ctx[b], INT_MAX - i) + i, lo = win_lo(pos, p.window), hi = min(pos, p.max_pos);
     row = (size_t)(row0 + i) * p.NQ + head;
     c0 = div_by(lo, a.part.C, a.Cm);
@@ -498,12 +509,12 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8CombArgs a) {
 }
 
 template <int NP>   // 2 (HD 128): the halves of the wave take the splits in turn
-__global__ void __launch_bounds__(256) kv8_combine_rows_kernel(const Kv8CombArgs a, int units) {
+__global__ void __launch_bounds__(256) kv8_combine_rows_kernel(const Kv8CombArgs a, int item0, unsigned units) {
     const Kv8Problem &p = a.p;
     const int HD = p.c.HD, lane = threadIdx.x & 63, per = HD > 256 ? HD / 256 : 1;
-    const int u = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6));
+    const unsigned u = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (u >= units) return;
-    const int bt = u / (p.NQ * per), hs = u - bt * p.NQ * per, head = hs / per;
+    const int it = (int)(u / (unsigned)(p.NQ * per)), hs = (int)u - it * p.NQ * per, head = hs / per, bt = item0 + it;
     size_t row;
     int c0, n;
     if (!comb_row(a, bt, head, row, c0, n)) return;
@@ -544,18 +555,25 @@ __global__ void __launch_bounds__(256) kv8_combine_rows_kernel(const Kv8CombArgs
 }
 
 hipError_t launch_kv8_combine(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st) {
-    const Kv8CombArgs a{p, part, div_magic(part.C)};
-    const long long units = (long long)p.B * p.T * p.NQ * (p.c.HD > 256 ? p.c.HD / 256 : 1);
-    // 3072 rows in up to 16 splits at HD 256: 12.8 us in workgroups, XX in waves; 128 rows in up to 64 at HD 512 5.0 and XX.
-    if (units >= 1024 && units <= INT_MAX) {
-        const dim3 g4((unsigned)((units + 3) / 4));
-        if (p.c.HD == 128) hipLaunchKernelGGL(kv8_combine_rows_kernel<2>, g4, dim3(256), 0, st, a, (int)units);
-        else hipLaunchKernelGGL(kv8_combine_rows_kernel<1>, g4, dim3(256), 0, st, a, (int)units);
+    const int per = p.c.HD > 256 ? p.c.HD / 256 : 1;
+    const bool by_row = p.cu && (long long)p.B * p.T > p.rows;        // (ragged rows: most of B * T are none)
+    const Kv8CombArgs a{p, part, div_magic(part.C), by_row ? 1 : 0};
+    const int items = by_row ? p.rows : p.B * p.T;
+    // 16 trees of 8 tokens x 24 q-heads in up to 16 splits at HD 256: 12.8 us in workgroups, 7.7 in waves.
+    if ((long long)items * p.NQ * per < 1024) {
+        hipLaunchKernelGGL(kv8_combine_kernel, dim3((unsigned)items, (unsigned)p.NQ, (unsigned)p.c.HD / 128), dim3(256), 0, st, a);
         return hipGetLastError();
     }
-    const dim3 grid((unsigned)p.B * (unsigned)p.T, (unsigned)p.NQ, (unsigned)p.c.HD / 128);
-    hipLaunchKernelGGL(kv8_combine_kernel, grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    const int most = (1 << 25) / (p.NQ * per);                         // items of a launch: 2^31 threads
+    for (int i0 = 0;; i0 += most) {
+        const int n = std::min(most, items - i0);
+        const unsigned units = (unsigned)n * (unsigned)(p.NQ * per);
+        const dim3 g4((units + 3) / 4);
+        if (p.c.HD == 128) hipLaunchKernelGGL(kv8_combine_rows_kernel<2>, g4, dim3(256), 0, st, a, i0, units);
+        else hipLaunchKernelGGL(kv8_combine_rows_kernel<1>, g4, dim3(256), 0, st, a, i0, units);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || items - i0 <= most) return e;
+    }
 }
 
 // ---------------------------------------------------------------- launch
@@ -621,7 +639,7 @@ hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, int n
     if (p.window > 0) per = std::min<long long>(per, ((long long)p.window + p.T - 2) / part.C + 2);
     const long long raw = per * p.B * p.c.NKV, units = a.nrg == 1 || raw < 64 ? raw : (raw + 7) / 8 * 8, wgs = units * a.nrg;
     if (a.nrg == 1 || raw < 64) a.spread = (int)raw;
-    if (wgs > INT_MAX) return hipErrorInvalidConfiguration;
+    if (!kv8_grid_ok(wgs, p.c.HD == 512 && nt > 1 ? 512 : 256)) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)wgs);
     switch (p.c.HD) {
     case 128: return nt == 1 ? launch_dec_n<128, 1>(a, grid, st) : nt == 2 ? launch_dec_n<128, 2>(a, grid, st) : launch_dec_n<128, 4>(a, grid, st);

@@ -1,9 +1,9 @@
 // Prompt attention over the paged 8-bit cache on gfx950: causal and sliding-window rows of ragged requests, behind any
 // cached prefix.
 //
-// A workgroup holds 64 RB query rows (token-major: tokens x q-heads of one KV head) and walks their keys in steps of 64 at
-// absolute positions. Its 8 waves are 4 row groups (16 RB rows each) x 2 key groups (32 keys of a step each); the two
-// states of a row are merged at the end through LDS.
+// A workgroup holds 64 or 128 query rows (token-major: tokens x q-heads of one KV head) and walks their keys in steps of 64
+// at absolute positions. Its waves are RG row groups of 16 RB rows x KG key groups, which share a step's keys; the states of a
+// row's key groups are merged at the end through LDS.
 //   * K and V pages go to LDS as codes, 16 bytes per lane straight from memory (global_load_lds), two stages, one barrier a
 //     step: half the LDS of 16-bit tiles, and half the bytes per fragment read. The 16-byte slots of a row are XOR-swizzled
 //     so that a fragment read meets every bank once (kf, vf below).
@@ -12,14 +12,17 @@
 //     lane group g then has the scores of keys 8 g .. 8 g + 7, which are the operand of O^T += V^T P^T as they stand, and
 //     V's [dim][token] rows give the other one: 8 bytes per lane. Q and the accumulators stay in registers.
 //   * Scales and softmax are those of the split-KV form (attn_kv8_decode.hip): the V scale is part of the weight.
-// Workgroups take a request's tiles from its last one on: the causal tiles with the most keys start first. Consecutive
+// Workgroups take the tiles of all requests from the latest on: the causal tiles with the most keys start first. Consecutive
 // workgroups take different KV heads, so that a head's pages are read through as few of the 8 L2s as there are heads for.
 //
 // Steps and key groups depend on positions alone and a step without keys for a row leaves its state as it was, so a row's
-// bits do not depend on its tile, its batch or how the prompt is cut; with key splits, on the split length too.
+// bits do not depend on its place in the tile or on the rest of the batch; they do on the tile's form, which is chosen by the
+// call's size, and with key splits on the split length.
 //
-// What bounds it: per step and wave 64 RB MFMAs, 16 RB conversions of the softmax's order and 256 of codes at HD 256. VALU and matrix
-// time are about equal at RB = 2 (a row group of 32).
+// What bounds it: the vector and the matrix pipe alternate. At HD 256 a wave of 32 rows takes, for 32 keys, 64 MFMAs of 16
+// cycles, 128 conversions of codes (each serves both row blocks) and about 350 other vector operations, most of them the
+// softmax; two waves per SIMD (registers) let one multiply while the other one converts. 6 requests of up to 2500 tokens, 24
+// q-heads over 4 of 256: 351 us, 855 TFLOP/s; 4096 tokens behind a window of 1024, 16 over 8: 90 us, 671 TFLOP/s.
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
@@ -458,7 +461,7 @@ static hipError_t launch_pre_k(const Kv8PrefArgs &a, hipStream_t st) {
     const long long G = a.p.NQ / a.p.c.NKV;
     const long long tiles = std::min((long long)a.p.B * ((a.p.T * G + Cf::RR - 1) / Cf::RR), (long long)a.p.rows * G / Cf::RR + a.p.B);
     const long long wgs = tiles * a.p.c.NKV * a.ns;
-    if (wgs > INT_MAX) return hipErrorInvalidConfiguration;
+    if (!kv8_grid_ok(wgs, Cf::NW * 64)) return hipErrorInvalidConfiguration;
     if constexpr (Cf::LDS > 64 * 1024) {                               // (per device; setting it again changes nothing)
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv8_prefill_kernel<HD, Cf, F16>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)Cf::LDS);

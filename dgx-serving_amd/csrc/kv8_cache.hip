@@ -407,9 +407,9 @@ hipError_t launch_kv8_append(const void *k, const void *v, int src_dtype, long k
     a.win = units <= 4096 ? 1 : units <= 32768 ? 4 : 16;
     a.windows = (rows - 1) / a.win + 1;
     const long long wgs = ((long long)a.windows * c.NKV + 7) / 8 * 8;
-    if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)wgs);
     const int threads = c.page * c.HD / 32;
+    if (!kv8_grid_ok(wgs, threads)) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)wgs);
     switch (src_dtype) {
     case DT_FP32: return launch_append_t<DT_FP32>(a, grid, threads, st);
     case DT_F16: return launch_append_t<DT_F16>(a, grid, threads, st);

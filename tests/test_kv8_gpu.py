@@ -394,6 +394,30 @@ def test_pages_outside_the_pool_are_not_attended(add):
     attn_case(15, "g2", 16, "bf16", [100, 50, 200], add, hurt=hurt, window=64)
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 0.0, -1.0])
+@pytest.mark.parametrize("add", [[1, 1, 1], [4, 4, 2], [100, 66, 1], [900, 1200, 1100]])
+def test_scales_of_pages_without_tokens_may_be_anything(add, scale):
+    """Scales that nobody has written, in pages that no row attends: those of nobody, page 0 in place of entries outside the
+    pool, and stale table entries behind the requests' last pages."""
+    def hurt(K, V, Ks, Vs, table):
+        spare = np.setdiff1d(np.arange(K.shape[0]), table)
+        if not (spare == 0).any():                                   # page 0 becomes a spare one
+            for x in (K, V, Ks, Vs):
+                x[spare[0]] = x[0]
+            table[table == 0] = spare[0]
+            spare[0] = 0
+        Ks[spare], Vs[spare] = scale, scale
+        K[spare], V[spare] = 0x7F, 0x7F
+        for b, n in enumerate(lens):
+            table[b, -(-n // 16):] = spare[-1]
+        table[0, 1] = -1
+        table[2, :3] = K.shape[0] + 7
+    ctx = [100, 50, 200]
+    lens = [c + a for c, a in zip(ctx, add)]
+    attn_case(23, "s4", 16, "bf16", ctx, add, hurt=hurt)
+    attn_case(24, "g2", 16, "f16", ctx, add, hurt=hurt)
+
+
 @pytest.mark.parametrize("ctx,add", [([-3, 5, -1], [1, 1, 1]), ([-3, 5, -1], [6, 2, 1]), ([-9, 5], [90, 70])])
 def test_rows_without_keys(ctx, add):
     """Positions below zero attend nothing and are written as such; requests without rows are not touched."""
