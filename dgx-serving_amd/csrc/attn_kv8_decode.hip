@@ -474,26 +474,36 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8CombArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, d4 = tid & 31, ph = tid >> 5, dim = (int)blockIdx.z * 128 + 4 * d4;
     const float *pm = a.part.m + row * a.part.ns + c0, *pl = a.part.l + row * a.part.ns + c0;
     const float *pa = a.part.acc + (row * a.part.ns + c0) * HD + dim;
-    float M = kNegInf;
-    for (int c = tid; c < n; c += 256) M = fmaxf(M, pm[c]);
+    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f}, t[4];
+    float M = kNegInf, L = 0.f, m0 = kNegInf, l0 = 0.f;
+    if (n > 0) {                                                       // the first splits, before their weights are known
+        m0 = pm[min(tid, n - 1)]; l0 = pl[min(tid, n - 1)];
+#pragma unroll
+        for (int x = 0; x < 4; x++) t[x] = *reinterpret_cast<const f32x4 *>(pa + (size_t)min(ph + 8 * x, n - 1) * HD);
+    }
+    M = m0;
+    for (int c = tid + 256; c < n; c += 256) M = fmaxf(M, pm[c]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
     if (lane == 0) part_s[0][wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(part_s[0][0], part_s[0][1]), fmaxf(part_s[0][2], part_s[0][3]));
-    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    float L = 0.f;
     for (int b0 = 0; b0 < n; b0 += 256) {
         if (b0) __syncthreads();
         if (b0 + tid < n) {
-            const float lc = pl[b0 + tid];
-            wt[tid] = kv8_weight(pm[b0 + tid], lc, M);
+            const float lc = b0 ? pl[b0 + tid] : l0;
+            wt[tid] = kv8_weight(b0 ? pm[b0 + tid] : m0, lc, M);
             L += lc * wt[tid];
         }
         __syncthreads();
         const int nb = min(256, n - b0);
+        if (b0 == 0) {
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                if (ph + 8 * x < nb) v += t[x] * wt[ph + 8 * x];
+        }
 #pragma unroll 4
-        for (int c = ph; c < nb; c += 8) v += *reinterpret_cast<const f32x4 *>(pa + (size_t)(b0 + c) * HD) * wt[c];
+        for (int c = b0 ? ph : ph + 32; c < nb; c += 8) v += *reinterpret_cast<const f32x4 *>(pa + (size_t)(b0 + c) * HD) * wt[c];
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
@@ -601,11 +611,13 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
         // Keys of a split, by the call's K and V in heads of 256 dims. Short ones leave a call to the prologues of its
         // workgroups and the merge, long ones to the longest workgroup. 16 requests of 9K keys x 4 heads (576K) took 42.8 us
         // in 256-key splits, 37.3 in 512 and 38.7 in 1024; of 32K keys (2M) 113.8 in 512 and 106.7 in 1024; 4 of 9K (144K)
-        // 19.7 in 256, 20.4 in 512 and 30.1 in 1024; one of 9K (36K) 13.0 in 128 and 15.2 in 256. With more than 16 rows the
+        // 19.7 in 256, 20.4 in 512 and 30.1 in 1024; one of 9K (36K) 13.0 in 128 and 15.2 in 256; 16 of up to 8K (524K) 25.7 in
+        // 256, 24.4 in 384 and 25.4 in 512, 8 of 9K (288K) 36.6, 32.7 and 36.1 (at HD 512
+        // 384 gains or loses by the lengths: 8 of up to 32K in two draws 26.0 and 30.4, 28.0 and 25.7 in 512). With more than 16 rows the
         // partials weigh more: 16 trees of 48 rows over 16K keys (1M) 87.7 us in 512 and 72.8 in 1024. Up to four steps go
         // without splits and their merge (9.5 us for 512 keys of 4 heads of 128, 10.4 in two splits).
         const long long work = (long long)B * NKV * keys * HD / 256;
-        if (chunk == 0) pl.C = work < 60000 ? 128 : work < 280000 ? 256 : work < (hr > 16 ? 700000 : 1500000) ? 512 : 1024;
+        if (chunk == 0) pl.C = work < 60000 ? 128 : work < 280000 ? 256 : work < 560000 && hr <= 16 && HD <= 256 ? 384 : work < (hr > 16 ? 700000 : 1500000) ? 512 : 1024;
         if (chunk == 0 && keys <= 512) pl.C = whole;
     } else {
         // Tiles of 64 rows. Where they do not fill the chip the split-KV form takes a prompt too: it walks 128 keys a step,
