@@ -711,9 +711,11 @@ hipError_t dgx_kv8_append(const void *k_src, const void *v_src, int src_dtype, l
 size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree) {
     if (!kv8_sizes_ok(B, T, rows, NQ, NKV, HD, max_pos, chunk)) return (size_t)-1;
     if (B == 0 || T == 0 || rows == 0) return 0;
-    const Kv8Plan pl = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window < 0 ? 0 : window, tree != 0);
-    if (pl.ns > 1 && !kv8_partials_ok(rows, NQ, pl.ns)) return (size_t)-1;
-    return pl.ns > 1 ? kv8_bytes((size_t)rows * NQ * pl.ns, HD) : 0;
+    if (window < 0) window = 0;
+    int ns = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, tree != 0).ns;
+    if (!tree && T <= 32) ns = std::max(ns, kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, true).ns);
+    if (ns > 1 && !kv8_partials_ok(rows, NQ, ns)) return (size_t)-1;
+    return ns > 1 ? kv8_bytes((size_t)rows * NQ * ns, HD) : 0;
 }
 
 hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,

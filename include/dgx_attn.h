@@ -273,8 +273,8 @@ hipError_t dgx_kv8_append(const void *k_src, const void *v_src, int src_dtype, l
 hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,
                         float *lse, int B, int T, int rows, int NQ, const int *ctx, const int *cu, const unsigned *anc, int max_pos,
                         int chunk, void *ws, size_t ws_bytes, hipStream_t st, float scale, int window);
-/* Bytes of ws for dgx_attn_kv8 with these sizes (tree: anc is given); grows with rows and max_pos / chunk. (size_t)-1 for
- * sizes that the call refuses. */
+/* Bytes of ws for dgx_attn_kv8 with these sizes; grows with rows and max_pos / chunk. tree 1: for calls with anc; 0: for calls
+ * without, and at T <= 32 for both. (size_t)-1 for sizes that the call refuses. */
 size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree);
 
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers). With timing on, the main

@@ -89,6 +89,19 @@ def test_workspace_holds_the_partials():
             A.attn_kv8_workspace(**d)
 
 
+def test_a_workspace_without_a_tree_holds_one_too():
+    """Runs of up to 32 tokens take a tree or not from step to step: the default size fits both."""
+    more = 0
+    for NQ, NKV, HD in ((24, 4, 256), (16, 1, 512), (16, 4, 128)):
+        for B in (1, 5, 16):
+            for T in (2, 11, 16, 32):
+                for max_pos in (300, 1200, 5000, 12000):
+                    both, tree = (A.attn_kv8_workspace(B, T, B * T, NQ, NKV, HD, max_pos, tree=t) for t in (False, True))
+                    assert both >= tree
+                    more += tree > 0
+    assert more
+
+
 def test_the_binding_refuses_wrong_tensors():
     f8 = torch.float8_e4m3fn
     K, V, S = torch.zeros(3, 2, 16, 128).to(f8), torch.zeros(3, 2, 128, 16).to(f8), torch.ones(3, 2)
