@@ -301,6 +301,9 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
                 }
             }
         }
+        // (From here to the step's end a wave goes before one at its scores: its workgroup waits for it at the barriers. 1024
+        // tokens causal 32.0 -> 29.6 us, tree verify 68.5 -> 66.3.)
+        __builtin_amdgcn_s_setprio(1);
         int vf0 = 0, vf1 = 0;
         if (s < s1) {
             vf0 = v_id(min(s + 2, s1), 0); vf1 = v_id(min(s + 2, s1), 1);
@@ -391,6 +394,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
             }
         }
         if (s < s1) { load_v(0, vn0); load_v(1, vn1); }
+        __builtin_amdgcn_s_setprio(0);
         vi0 = vn0; vi1 = vn1; vn0 = vf0; vn1 = vf1;
         cur = next; nxt = n2; sn = s2; okn = own_ok(next);
     }
