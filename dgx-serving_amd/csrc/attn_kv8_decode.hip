@@ -625,14 +625,16 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
         if (chunk == 0 && keys <= 512) pl.C = whole;
     } else {
         // Tiles of 64 rows. Where they do not fill the chip the split-KV form takes a prompt too: it walks 128 keys a step,
-        // and its row groups can be smaller and its keys split.
+        // and its row groups can be smaller and its keys split. Split-KV | tiles, us: causal 1400 x 16 q-heads over 8 (352
+        // tiles) 43.4 | 47.6, 1024 x 24 over 4 (384) 42.9 | 39.2, 800 x 24 behind 2000 (300) 112.6 | 85.8, 1000 x 16 over 8
+        // behind 2000 (250) 75.8 | 79.0; behind a window of 1024 500 x 16 over 8 (125) 35.2 | 38.2, 600 (150) 41.9 | 38.8; HD 512
+        // 800 x 16 (200) 42.7 | 46.7, 1024 (256) 57.1 | 54.2.
         const long long n64 = std::min((long long)B * ((hr + 63) / 64), (long long)rows * G / 64 + B) * NKV;
-        pl.prefill = n64 >= 400;
+        pl.prefill = n64 >= (HD == 512 ? 250 : window > 0 && window <= max_pos ? 140 : keys <= 2304 ? 360 : 280);
         if (!pl.prefill) {
-            // 200 x 16 q-heads over 8 without a prefix: groups of 16 rows 9.5 us, 32 12.2, 64 16.9, the tile kernel 11.4;
-            // 1000 behind 1000: 72, 53, 64 and 60; 512 behind 4096: 64 rows in 1536-key splits 74, in 1024 87, no split of 16
-            // rows 93, the tile kernel in 1024-key splits 85. Fewer workgroups at HD 512: 500 x 16 over 1 behind 4000 117
-            // us unsplit, 138 in 1536; 100 behind 4000 41 in 1024, 52 in 512.
+            // 200 x 16 q-heads over 8 without a prefix: groups of 16 rows 9.5 us, 32 12.2, 64 16.9; 1000 behind 1000: 72, 53 and
+            // 64; 512 behind 4096: 64 rows in 1536-key splits 74, in 1024 87, no split of 16 rows 93. Fewer workgroups at HD
+            // 512: 500 x 16 over 1 behind 4000 117 us unsplit, 138 in 1536; 100 behind 4000 41 in 1024, 52 in 512.
             const long long n = HD == 512 ? n64 * 2 : n64, want = HD == 512 ? 200 : 450;
             pl.nt = HD == 512 ? 2 : 4;
             if (chunk == 0 && keys <= 1280) pl.nt = 1, pl.C = whole;

@@ -19,10 +19,10 @@
 // bits do not depend on its place in the tile or on the rest of the batch; they do on the tile's form, which is chosen by the
 // call's size, and with key splits on the split length.
 //
-// What bounds it: the vector and the matrix pipe alternate. At HD 256 a wave of 32 rows takes, for 32 keys, 64 MFMAs of 16
-// cycles, 128 conversions of codes (each serves both row blocks) and about 350 other vector operations, most of them the
+// What bounds it: the vector and the matrix pipe share the issue slots. At HD 256 a wave of 32 rows takes, for 32 keys, 64 MFMAs
+// of 16 cycles, 128 conversions of codes (each serves both row blocks) and about 120 other vector operations, most of them the
 // softmax; two waves per SIMD (registers) let one multiply while the other one converts. 6 requests of up to 2500 tokens, 24
-// q-heads over 4 of 256: 351 us, 855 TFLOP/s; 4096 tokens behind a window of 1024, 16 over 8: 90 us, 671 TFLOP/s.
+// q-heads over 4 of 256: 325 us, 924 TFLOP/s; 4096 tokens behind a window of 1024, 16 over 8: 80 us, 755 TFLOP/s.
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
@@ -263,7 +263,12 @@ __global__ void __launch_bounds__(Cf::NW * 64, Cf::OCC) kv8_prefill_kernel(const
         // (Scalar loads without a branch around them, taken over at the end of the step: they wait with the stage.)
         const Scales s2 = scales_of(nxt);
         const Ids n2 = ids_of(min(s + 2, s_hi));
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // stage s has landed, from every wave
+        // Stage s has landed, from every wave. By the builtin, not asm: the compiler then knows that the Q and page id loads
+        // have landed too, and does not wait for them, and with them for the next stage, at their uses (2048 tokens causal, 16
+        // q-heads over 8, 76.2 -> 64.4 us; HD 512 295 -> 275). With two sub-steps a step is long enough for that not to
+        // matter, and its registers suffer (HD 128 93 -> 98).
+        if constexpr (NSUB == 1) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt 0
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         const Scales &sc = sn;
         const VIds vcur = vnxt;
@@ -338,9 +343,10 @@ __global__ void __launch_bounds__(Cf::NW * 64, Cf::OCC) kv8_prefill_kernel(const
                 float mx = tv[0];
 #pragma unroll
                 for (int i = 1; i < 8; i++) mx = fmaxf(mx, tv[i]);
-                mx = max_over_groups(__builtin_fmaf(mx, f, ev));
-                const float mn = mx > m[rb] + move ? mx - head : m[rb];
-                if (__any(mn != m[rb])) {
+                mx = __builtin_fmaf(mx, f, ev);
+                if (__any(mx > m[rb] + move)) {                         // rare: only then the lane groups' maxima meet
+                    mx = max_over_groups(mx);
+                    const float mn = mx > m[rb] + move ? mx - head : m[rb];
                     const float al = mn == m[rb] ? 1.f : fast_exp2(m[rb] - mn);
                     l[rb] *= al; m[rb] = mn;
 #pragma unroll
@@ -501,14 +507,14 @@ hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, hipS
         a.ns = (int)std::max(2ll, per);
     }
     // Tiles of 128 rows where there are two rounds of them for the 512 workgroups that run at once (one, under a window: its
-    // tiles are equally long), else of 64. HD 256, TFLOP/s of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400
-    // tiles of 128) 853 | 732, 4096 behind a window of 1024, 16 over 8 (512 tiles) 666 | 598, causal 4000 of those (500) 604 | 776.
+    // tiles are equally long), else of 64. HD 256, us of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400 tiles
+    // of 128) 326 | 361, 4096 behind a window of 1024, 16 over 8 (512) 79.7 | 87.9, causal 4096 of those (512) 202 | 153.
     const long long rows = std::min((long long)p.B * p.T, (long long)p.rows) * G * p.c.NKV * a.ns;
     const bool wide = rows >= 128 * (p.window > 0 && p.window < p.max_pos ? 500 : 960);
     switch (p.c.HD) {
     case 128: return wide ? launch_pre<128, Kv8PrefCfg<128, 2, 4, 1, 2, 2>>(a, st) : launch_pre<128, Kv8PrefCfg<128, 2, 2, 2, 1, 3>>(a, st);
     case 256: return wide ? launch_pre<256, Kv8PrefCfg<256, 2, 4, 1, 2, 2>>(a, st) : launch_pre<256, Kv8PrefCfg<256, 2, 2, 2, 1, 2>>(a, st);
-    case 512:                                                          // (64 rows in 8 waves: 4 of 1500 x 16 q-heads 299 us, in 4 waves 333, 32 rows 444)
+    case 512:                                                          // (64 rows in 8 waves; before later steps 4 of 1500 x 16 q-heads 299 us, in 4 waves 333, 32 rows 444; 275 now)
         return launch_pre<512, Kv8PrefCfg<512, 1, 4, 2, 1, 2>>(a, st);
     default: return hipErrorInvalidValue;
     }
