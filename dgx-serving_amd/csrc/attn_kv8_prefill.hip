@@ -6,7 +6,8 @@
 // row's key groups are merged at the end through LDS.
 //   * K and V pages go to LDS as codes, 16 bytes per lane straight from memory (global_load_lds), two stages, one barrier a
 //     step: half the LDS of 16-bit tiles, and half the bytes per fragment read. The 16-byte slots of a row are XOR-swizzled
-//     so that a fragment read meets every bank once (kf, vf below).
+//     (kf, vf below): K's 16-byte fragment reads meet every bank once, V's 8-byte ones take two turns, a third of the LDS
+//     pipe's time in all.
 //   * Fragments are converted to 16 bits (exact) as they are read; every conversion serves the wave's 16 RB rows.
 //   * S^T = K Q^T on 16x16x32 with tile t (of 2) of a wave's 32 keys holding key 8 (rho / 4) + 4 t + rho % 4 in row rho:
 //     lane group g then has the scores of keys 8 g .. 8 g + 7, which are the operand of O^T += V^T P^T as they stand, and

@@ -13,10 +13,11 @@ namespace dgx {
 // All or nothing: a step that needs more free pages, columns or rows than there are, or has a negative length, takes nothing
 // (status tells which), gives every row slot -1 and every request no rows.
 //
-// Bound by latency: lengths, scan, free ids, slots. The scans take one workgroup's time whatever the grid, so every workgroup
-// does them (lengths come from the L2) and takes its share of the rows; a second launch behind a one-workgroup scan would
+// Bound by latency: lengths, scan, free ids, slots (256 requests of one token 3.1 us, 96 prompts of 123K rows in all 5.9). The
+// scans take one workgroup's time whatever the grid, so every workgroup does them (lengths come from the L2) and takes its
+// share of the rows, from 2048 each on: 96 prompts 98 us in one workgroup. A second launch behind a one-workgroup scan would
 // cost more than the scan. One workgroup alone does it all where the free count is updated in place (another workgroup
-// could read it late), and for up to 8192 rows.
+// could read it late).
 struct PlanArgs {
     const int *ctx, *add, *free_pages, *free_in;
     int *table, *free_out, *cu, *slots, *status;
@@ -142,8 +143,8 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
                            const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots, int rows,
                            int *status, hipStream_t st) {
     const PlanArgs a{ctx, add, free_pages, free_in, table, free_out, cu, slots, status, table_stride, B, lp, cols, rows, free_cap};
-    const int grid = free_in == free_out || rows <= 8192 ? 1 : std::min(128, (rows + 2047) / 2048);
-    const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;     // fewer waves meet sooner at the barriers
+    const int grid = free_in == free_out || rows <= 2048 ? 1 : std::min(128, (rows + 2047) / 2048);
+    const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;     // fewer waves meet sooner at the barriers (4.5 us a call, 5.1 with 1024)
     if (rows <= kNarrow && cols <= kNarrow) hipLaunchKernelGGL(kv8_plan_kernel<int>, dim3(grid), dim3(threads), 0, st, a);
     else hipLaunchKernelGGL(kv8_plan_kernel<long long>, dim3(grid), dim3(threads), 0, st, a);
     return hipGetLastError();
@@ -161,7 +162,8 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
 // A token with a value that is not finite gets K codes NaN and 0 in place of V's values that are not finite: a score with it
 // is NaN, so every row that attends it comes out NaN, and rows that do not are left alone (a NaN code in V would reach the
 // other rows of a matrix tile through 0 * NaN).
-// Bound by memory: 60K rows x 8 heads x 256 from bf16 read 2 bytes and write 1 per element.
+// Bound by memory: 66K rows x 8 heads x 256 from bf16 read 2 bytes and write 1 per element, 172 us, 4.74 TB/s (a large copy
+// reaches 4.82). Small calls by latency: 16 rows of a token each 5.4 us, a prompt of 1024 from fp32 9.8.
 struct AppendArgs {
     const void *k, *v;
     long ks, vs;                      // row strides in elements
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const AppendArgs a) {
     using SE = typename Elem<ST>::T;
     extern __shared__ __align__(16) unsigned char tile[];          // V codes of the run, [HD][page], swizzled
     __shared__ float red[2][16];
-    __shared__ int bad_s[64], nonfin[2];
+    __shared__ int bad_s[64], nonfin[2], rows_s[64];
     const Kv8 &c = a.c;
     const int page = c.page, HD = c.HD, PQ = page / 4;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, nw = (nt + 63) >> 6;
@@ -215,22 +217,46 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const AppendArgs a) {
     if (unit / (unsigned)c.NKV >= (unsigned)a.windows) return;
     const int w0 = (int)(unit / (unsigned)c.NKV) * a.win;
     const int total = c.pages << c.lp;                             // host: at most INT_MAX
+    auto slot_of = [&](int r) { return (unsigned)r < (unsigned)a.rows ? a.slots[r] : -1; };
+    // A row begins a run unless the last row before it that is not skipped holds the token before its own, in the same page.
     unsigned long long starts;
     {
-        const int r = w0 + lane;
-        const bool in = lane < a.win && r < a.rows;
-        const int s = in ? a.slots[r] : -1, prev = in && r > 0 ? a.slots[r - 1] : -2;
-        starts = __ballot(s >= 0 && s < total && !(prev == s - 1 && (s & (page - 1)) != 0));
+        const int r = w0 + lane, s = lane < a.win ? slot_of(r) : -1, prev = lane < a.win ? slot_of(r - 1) : -1;
+        const bool ok = (unsigned)s < (unsigned)total, inner = (s & (page - 1)) != 0;
+        starts = __ballot(ok && !(prev == s - 1 && inner));
+        if (__ballot(ok && inner && r > 0 && (unsigned)prev >= (unsigned)total)) {   // rare: skipped rows to look behind
+            const int s2 = slot_of(w0 - (64 - a.win) + lane);          // the window's rows are the last lanes'
+            const bool ok2 = (unsigned)s2 < (unsigned)total;
+            const unsigned long long below = __ballot(ok2) & ((1ull << lane) - 1);
+            const int last = __shfl(s2, below ? 63 - __builtin_clzll(below) : lane);
+            starts = __ballot(ok2 && lane >= 64 - a.win && !(below && last == s2 - 1 && (s2 & (page - 1)) != 0)) >> (64 - a.win);
+        }
     }
     const int dv = tid & ((1 << a.lv) - 1), tg = tid >> a.lv;      // 8 dims from 8 dv, tokens 4 tg .. 4 tg + 3 of the run
     for (; starts; starts &= starts - 1) {
         const int r0 = w0 + __builtin_ctzll(starts), s0 = __builtin_amdgcn_readfirstlane(a.slots[r0]);
         const int off = s0 & (page - 1), pid = s0 >> c.lp;
+        // Its n tokens: the rows from r0 on with the slots s0, s0 + 1, .. within the page; skipped rows may lie between them.
         int n;
+        bool dense = true;                                             // none do
         {
-            const int sl = r0 + lane < a.rows ? a.slots[r0 + lane] : -1;
-            const unsigned long long ok = __ballot(sl == s0 + lane && off + lane < page);
-            n = ~ok ? __builtin_ctzll(~ok) : 64;
+            const int sa = slot_of(r0 + lane);
+            const unsigned long long next = ~__ballot(sa == s0 + lane && off + lane < page);
+            n = next ? __builtin_ctzll(next) : 64;
+            if (off + n < page && (n == 64 || (__ballot((unsigned)sa >= (unsigned)total) >> n & 1)) && r0 + n < a.rows) {   // rare: a skipped row is next
+                const unsigned long long under = (1ull << lane) - 1;
+                int k = 0;
+                for (int part = 0; part < 2; part++) {
+                    const int sx = part ? slot_of(r0 + 64 + lane) : sa, kx = k + __popcll(__ballot((unsigned)sx < (unsigned)total) & under);
+                    const bool taken = (unsigned)sx < (unsigned)total, in = sx == s0 + kx && off + kx < page;
+                    const unsigned long long stop = __ballot(taken && !in), mine = __ballot(taken && in) & (stop ? (stop & -stop) - 1 : ~0ull);
+                    if (mine >> lane & 1) rows_s[kx] = 64 * part + lane;
+                    k += __popcll(mine);
+                    if (stop) break;
+                }
+                dense = k == n;
+                n = k;
+            }
         }
         for (int i = tid; i < 64; i += nt) bad_s[i] = 0;
         if (tid < 2) nonfin[tid] = 0;
@@ -238,11 +264,18 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const AppendArgs a) {
         Src8<ST> x[2][4];
         const bool live = 4 * tg < n;
         if (live) {
+            int row[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) row[i] = min(4 * tg + i, n - 1);
+            if (!dense) {                                              // (all waves write the same rows_s and each reads what it wrote)
+#pragma unroll
+                for (int i = 0; i < 4; i++) row[i] = rows_s[row[i]];
+            }
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const SE *p = reinterpret_cast<const SE *>(t ? a.v : a.k) + (size_t)(r0 + min(4 * tg + i, n - 1)) * (size_t)(t ? a.vs : a.ks) + h * HD + 8 * dv;
+                    const SE *p = reinterpret_cast<const SE *>(t ? a.v : a.k) + (size_t)(r0 + row[i]) * (size_t)(t ? a.vs : a.ks) + h * HD + 8 * dv;
 #pragma unroll
                     for (int q = 0; q < (ST == DT_FP32 ? 2 : 1); q++) x[t][i].w[q] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p) + q);
                 }
@@ -401,8 +434,10 @@ hipError_t launch_kv8_append(const void *k, const void *v, int src_dtype, long k
                              const int *slots, int rows, unsigned *stats, hipStream_t st) {
     AppendArgs a{k, v, k_stride, v_stride, c, slots, stats, rows, 1, 0, 0};
     while ((8 << a.lv) < c.HD) a.lv++;
-    // A workgroup looks for runs among `win` rows. One row each while the rows are few (a decode step's rows are runs of
-    // one, and a window's runs are taken one after another); more for prompts, where most workgroups would find none.
+    // A workgroup looks for runs among `win` rows, and takes those that begin there one after another. Windows of 1 | 4 | 16
+    // rows, us: 16 requests of a token x 4 heads (64 units) 5.9 | 13.8 | 45.9, 256 of a token x 4 (1024) 13.6 | 16.2 | 46.0, 512
+    // of up to 4 x 8 (10K) 58.7 | 50.1 | 62.6, a prompt of 1024 x 8 (8K) 15.6 | 12.1 | 15.6, 66K rows of prompts x 8 (532K) 364 |
+    // 211 | 172: most workgroups of a prompt find none.
     const long long units = (long long)rows * c.NKV;
     a.win = units <= 4096 ? 1 : units <= 32768 ? 4 : 16;
     a.windows = (rows - 1) / a.win + 1;

@@ -247,9 +247,10 @@ hipError_t dgx_kv8_plan(const int *ctx, const int *add, int B, int page, int *ta
                         int *status, hipStream_t st);
 
 /* Append rows r = 0 .. rows - 1 of k_src and v_src ([NKV, HD] each, fp32 / f16 / bf16, k_stride and v_stride elements between
- * rows: multiples of 16 bytes, 16-byte aligned) at slots[r]; rows with a slot outside [0, pages * page) are skipped. Rows of
- * one page follow each other, in ascending slots, in one call (as dgx_kv8_plan's slots do), and no page is written by two
- * requests or two overlapping calls.
+ * rows: multiples of 16 bytes, 16-byte aligned) at slots[r]; rows with a slot outside [0, pages * page) are skipped. The
+ * rows of one page in a call hold consecutive slots and follow each other (as dgx_kv8_plan's do), with at most 32 skipped rows
+ * between the first and the last of them (drafts that were not accepted, say), and no page is written by two requests or two
+ * overlapping calls.
  * The page's scale becomes the least that holds the new rows and is at least its own, unless the rows begin at the page's
  * token 0; the codes of earlier tokens are rounded again when it grows (exact but for codes that become smaller than 2^-6
  * scales). Tokens behind the new rows keep their bytes. A token with a non-finite value in a head gets NaN codes in that

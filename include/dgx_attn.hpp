@@ -198,4 +198,33 @@ static inline void launch_flash_attn_v2(const float *Q, const KV *Kc, const KV *
                       "flash_v2");
 }
 
+// ---- paged 8-bit cache (no reference counterpart; the arguments are those of dgx_attn.h)
+static inline void kv8_plan(const int *ctx, const int *add, int B, int page, int *table, long table_stride, int table_cols,
+                            const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots,
+                            int rows, int *status, hipStream_t st = 0) {
+    dgx_detail::check(dgx_kv8_plan(ctx, add, B, page, table, table_stride, table_cols, free_pages, free_cap, free_in, free_out,
+                                   cu, slots, rows, status, st),
+                      "kv8_plan");
+}
+template <typename T>
+static inline void kv8_append(const T *k, const T *v, long k_stride, long v_stride, const dgx_kv8 &cache, const int *slots,
+                              int rows, hipStream_t st = 0) {
+    dgx_detail::check(dgx_kv8_append(k, v, dgx_detail::kv_code<T>(), k_stride, v_stride, &cache, slots, rows, st), "kv8_append");
+}
+static inline size_t attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk = 0,
+                                        int window = 0, bool tree = false) {
+    const size_t n = dgx_attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, tree ? 1 : 0);
+    dgx_detail::check(n == (size_t)-1 ? hipErrorInvalidValue : hipSuccess, "attn_kv8 workspace");
+    return n;
+}
+template <typename TQ, typename TO>
+static inline void launch_attn_kv8(const TQ *Q, const dgx_kv8 &cache, const int *table, long table_stride, TO *O, int B, int T,
+                                   int rows, int NQ, const int *ctx, const int *cu, int max_pos, void *ws, size_t ws_bytes,
+                                   hipStream_t st = 0, const unsigned *anc = nullptr, float scale = 0.f, int window = 0,
+                                   float *lse = nullptr, int chunk = 0) {
+    dgx_detail::check(dgx_attn_kv8(Q, dgx_detail::kv_code<TQ>(), &cache, table, table_stride, O, dgx_detail::kv_code<TO>(), lse,
+                                   B, T, rows, NQ, ctx, cu, anc, max_pos, chunk, ws, ws_bytes, st, scale, window),
+                      "attn_kv8");
+}
+
 #endif  // DGX_ATTN_HPP

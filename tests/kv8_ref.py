@@ -42,12 +42,12 @@ def append(K, V, Ks, Vs, k, v, slots):
     """The append of rows k, v [rows, NKV, HD] (float64) on code arrays K [P, NKV, page, HD], V [P, NKV, HD, page] and scales,
     in place."""
     P, NKV, page, HD = K.shape
+    slots = np.asarray(slots)
+    taken = (slots >= 0) & (slots < P * page)
+    k, v, slots = k[taken], v[taken], slots[taken]
     r = 0
     while r < len(slots):
         s = int(slots[r])
-        if not 0 <= s < P * page:
-            r += 1
-            continue
         n = 1
         while r + n < len(slots) and slots[r + n] == s + n and (s + n) % page:
             n += 1

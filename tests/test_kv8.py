@@ -119,6 +119,42 @@ def test_the_binding_refuses_wrong_tensors():
         A.kv8_plan(i, i, 16, torch.zeros(2, 3, dtype=torch.int32), i, i[:1], i[:1], torch.zeros(3, dtype=torch.int32), i, i[:1])
 
 
+CALLER = r"""
+#include "dgx_attn.hpp"
+#include <cstdio>
+int main(int argc, char **) {
+    dgx_kv8 c{(void *)16, (void *)16, (float *)16, (float *)16, 8, 64, 4, 256};
+    launch_attn_kv8<__half, float>(nullptr, c, nullptr, 0, nullptr, 0, 1, 0, 24, nullptr, nullptr, 100, nullptr, 0);
+    launch_attn_kv8<__hip_bfloat16, __hip_bfloat16>(nullptr, c, nullptr, 0, nullptr, 2, 1, 0, 24, nullptr, nullptr, 100, nullptr, 0);
+    kv8_append<float>(nullptr, nullptr, 1024, 1024, c, nullptr, 0);
+    printf("%d %d\n", attn_kv8_workspace(1, 1, 1, 24, 4, 256, 63) == 0, attn_kv8_workspace(16, 1, 16, 24, 4, 256, 8191) > 0);
+    fflush(stdout);
+    if (argc > 1) kv8_plan(nullptr, nullptr, 1, 48, nullptr, 0, 0, nullptr, 0, nullptr, nullptr, nullptr, nullptr, 0, nullptr);
+    return 0;
+}
+"""
+
+
+def test_cxx_callers(tmp_path):
+    """The C++ names compile, link and run; a refused call ends the process with its name, as the other launchers do."""
+    import os
+    import signal
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.join(root, "dgx-serving_amd")
+    (tmp_path / "caller.cpp").write_text(CALLER)
+    exe = str(tmp_path / "caller")
+    cmd = ["/opt/rocm/bin/amdclang++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(root, "include"), "-I", "/opt/rocm/include",
+           str(tmp_path / "caller.cpp"), "-o", exe, "-L", lib, "-ldgx_attn", "-L", "/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{lib}:/opt/rocm/lib"]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-3000:]
+    env = {k: v for k, v in os.environ.items() if not k.startswith("G4_")}
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=60, env=env)
+    assert out.returncode == 0 and out.stdout.split() == ["1", "1"], out.stderr
+    bad = subprocess.run([exe, "x"], capture_output=True, text=True, timeout=60, env=env)
+    assert bad.returncode == -signal.SIGABRT and "[kv8_plan] failed" in bad.stderr, (bad.returncode, bad.stderr)
+
+
 def test_reference_codes_are_torchs():
     """The tests' encoder against torch's cast, and its decoder against torch's values."""
     rng = np.random.default_rng(0)

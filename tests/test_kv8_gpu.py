@@ -101,6 +101,23 @@ def test_plan_lengths_near_2_31():
 
 
 # ---------------------------------------------------------------- append
+def test_plan_of_more_rows_than_32_bit_scans_hold():
+    """Room for more than 2^20 rows: the wide scans, over more requests than a tile's 1024."""
+    rng = np.random.default_rng(8)
+    B, page, rows = 1500, 64, (1 << 20) + 777
+    ctx, add = rng.integers(0, 300, B), rng.integers(0, 900, B)
+    need = int((-(-(ctx + add) // page) - -(-ctx // page)).sum())
+    free = rng.permutation(need + 3)
+    table = np.full((B, 20), -7)
+    have = -(-ctx // page)
+    for b in range(B):
+        table[b, :have[b]] = 500 + b
+    for in_place in (False, True):
+        got = run_plan(ctx, add, page, table, free, len(free), rows, in_place)
+        for g, w in zip(got, ref_plan(ctx, add, page, table, free, len(free), rows)):
+            assert np.array_equal(g, w)
+
+
 def values(rng, rows, NKV, HD, dtype, sd=1.0):
     """Rows as the source type stores them: (tensor on the GPU, float64)."""
     t = torch.from_numpy(rng.standard_normal((rows, NKV, HD)) * sd).to(R.DTYPES[dtype])
@@ -205,6 +222,51 @@ def test_append_strided_rows_of_a_fused_projection_and_many_rows():
     R.append(K, V, Ks, Vs, k.double().cpu().numpy(), v.double().cpu().numpy(), slots)
     A.kv8_append(k, v, cache, i32(slots))
     same_cache(cache, K, V, Ks, Vs)
+
+
+@pytest.mark.parametrize("B,NKV,top", [(700, 8, 1), (900, 8, 3), (900, 16, 5), (9000, 4, 1)])
+def test_append_of_many_short_runs(B, NKV, top):
+    """Windows of 4 and 16 rows that hold many runs each: requests of a few tokens, some behind others of their page."""
+    rng = np.random.default_rng(B)
+    page, HD = 16, 128
+    have, add = rng.integers(0, page - top, B), rng.integers(1, top + 1, B)
+    K, V, Ks, Vs = R.make_cache(rng, B, page, NKV, HD)
+    cache = R.to_cache(A, K, V, Ks, Vs)
+    slots = np.concatenate([p * page + h + np.arange(n) for p, h, n in zip(rng.permutation(B), have, add)])
+    slots = np.insert(slots, rng.integers(0, len(slots), len(slots) // 10), -1)
+    assert len(slots) * NKV > 4096
+    kt, k = values(rng, len(slots), NKV, HD, "bf16", 3.0)
+    vt, v = values(rng, len(slots), NKV, HD, "bf16", 0.1)
+    A.kv8_append(kt, vt, cache, i32(slots))
+    R.append(K, V, Ks, Vs, k, v, slots)
+    same_cache(cache, K, V, Ks, Vs)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_append_with_skipped_rows_between_a_pages_rows(page):
+    """Rows of one page with up to 32 skipped ones between them (drafts that were not accepted), in windows of 1, 4 and 16 rows:
+    one run, so the scale is the least that holds all of them and every code is rounded once."""
+    rng = np.random.default_rng(page)
+    for NKV, runs in ((1, 6), (2, 60), (16, 150)):
+        HD, slots = 128, []
+        for pid in rng.permutation(runs):
+            off = int(rng.integers(0, page))
+            n = int(rng.integers(1, page - off + 1))
+            rows = np.full(n + int(rng.integers(0, 33)), -1)
+            at = np.sort(rng.choice(len(rows) - 2, n - 2, replace=False) + 1) if n > 2 else np.array([], int)
+            at = np.concatenate([[0], at, [len(rows) - 1]])[:n] if n > 1 else np.array([0])
+            rows[at] = pid * page + off + np.arange(n)
+            rows[rows < 0] = rng.choice([-1, runs * page, 1 << 30], (rows < 0).sum())
+            slots += list(rows) + [-5] * int(rng.integers(0, 70) if rng.random() < 0.2 else 0)
+        K, V, Ks, Vs = R.make_cache(rng, runs, page, NKV, HD)
+        cache = R.to_cache(A, K, V, Ks, Vs)
+        kt, k = values(rng, len(slots), NKV, HD, "f16", 2.0)
+        scale = torch.from_numpy(2.0 ** rng.integers(-3, 4, len(slots))).to(kt).view(-1, 1, 1)
+        kt = kt * scale
+        A.kv8_append(kt, kt, cache, i32(slots))
+        k = kt.double().cpu().numpy()
+        R.append(K, V, Ks, Vs, k, k, slots)
+        same_cache(cache, K, V, Ks, Vs, f"{NKV} heads, {len(slots)} rows")
 
 
 # ---------------------------------------------------------------- attention
