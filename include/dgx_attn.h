@@ -241,7 +241,8 @@ typedef struct dgx_kv8 {
  * status[0] = 0, or a sum of 1: too few free pages, 2: a request needs more than table_cols pages, 4: more than `rows` new
  * tokens, 8: a negative length or a count outside [0, free_cap]. Then the step takes nothing: table and count stay as they
  * are, every slot is -1 and cu is zero (an append and an attention call over them do nothing).
- * To give pages back, write their ids over free_pages[count ..] and raise the count. */
+ * To give pages back, write their ids over free_pages[count ..] and raise the count; a request whose ctx is lowered (drafts that
+ * were not accepted) has to give back those behind its first ceil(ctx / page), or they are lost. */
 hipError_t dgx_kv8_plan(const int *ctx, const int *add, int B, int page, int *table, long table_stride, int table_cols,
                         const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots, int rows,
                         int *status, hipStream_t st);
@@ -269,12 +270,12 @@ hipError_t dgx_kv8_append(const void *k_src, const void *v_src, int src_dtype, l
  * what O and lse hold.
  * chunk: keys of a split (a multiple of 64; 0: chosen from the sizes). ws: dgx_attn_kv8_workspace bytes for the same
  * sizes, 16-byte aligned, used by this call alone until it has run (calls on other streams and other graphs take their
- * own). Results do not depend on the other requests of a batch, but the choices made from B, T and max_pos do.
+ * own). Results do not depend on the other requests of a batch, but the forms chosen from B, T, rows and max_pos do.
  * hipErrorInvalidValue for sizes or types outside the above, or a workspace that is too small. */
 hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,
                         float *lse, int B, int T, int rows, int NQ, const int *ctx, const int *cu, const unsigned *anc, int max_pos,
                         int chunk, void *ws, size_t ws_bytes, hipStream_t st, float scale, int window);
-/* Bytes of ws for dgx_attn_kv8 with these sizes; grows with rows and max_pos / chunk. tree 1: for calls with anc; 0: for calls
+/* Bytes of ws for dgx_attn_kv8 with these sizes (others, smaller ones too, may take another form and need more). tree 1: for calls with anc; 0: for calls
  * without, and at T <= 32 for both. (size_t)-1 for sizes that the call refuses. */
 size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree);
 

@@ -271,7 +271,7 @@ def test_append_with_skipped_rows_between_a_pages_rows(page):
 
 # ---------------------------------------------------------------- attention
 HEADS = {"q6": (24, 4, 256), "g2": (4, 2, 256), "g16": (16, 1, 512), "s4": (8, 2, 128), "g1": (2, 2, 128), "g5": (5, 1, 512), "g3": (6, 2, 128),
-         "g20": (20, 1, 256)}
+         "g20": (20, 1, 256), "g96": (96, 1, 128), "g130": (130, 1, 256)}
 
 
 def attn_case(seed, heads, page, io, ctx, add, window=0, tree=False, chunk=0, out=None, spread=2, uniform=False, scale=0.0, hurt=None,
@@ -391,6 +391,16 @@ def test_every_form_of_prompts(form):
     for r, b in zip(some, seq):
         one = R.attention(Q[r:r + 1].double().numpy(), K, V, Ks, Vs, table[b:b + 1], [int(ctx[b] + r - cu[b])], np.array([0, 1]), window=window)
         R.check(O[r:r + 1], lse[r:r + 1], one, f"{form}, row {r}")
+
+
+@pytest.mark.parametrize("heads,add", [("g96", [1, 1]), ("g130", [1, 0, 1]), ("g96", [5, 3]), ("g130", [7, 32]), ("g96", [150, 110]), ("g130", [3, 190])])
+def test_more_heads_than_a_tiles_rows(heads, add):
+    """Groups of 96 and 130 q-heads: a token's rows lie in several tiles, in every form."""
+    ctx = [130, 7, 61][:len(add)]
+    attn_case(26, heads, 16, "f16", ctx, add)
+    attn_case(27, heads, 64, "bf16", ctx, add, window=70)
+    if max(add) <= 32:
+        attn_case(28, heads, 32, "bf16", ctx, add, tree=True, chunk=64)
 
 
 def test_prompts_of_many_requests():
