@@ -35,11 +35,11 @@ HEADS = {"qwen": (24, 4, 256), "slide": (16, 8, 256), "global": (16, 1, 512), "s
 
 
 def _lib():
-    lib = sys.modules.get("dgx_attn")
-    if lib is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dgx-serving_amd"))
-        import dgx_attn as lib
-    return lib
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dgx-serving_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import dgx_attn
+    return dgx_attn
 
 
 def _case(kind, B, lo, hi, tlo, thi, page=64, heads="qwen", io="f16", src="bf16", window=0, tree=False, chunk=0, lens=1, name=None):
