@@ -718,6 +718,18 @@ size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, i
     return ns > 1 ? kv8_bytes((size_t)rows * NQ * ns, HD) : 0;
 }
 
+hipError_t dgx_attn_kv8_form(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree, int form[4]) {
+    if (!form || !kv8_sizes_ok(B, T, rows, NQ, NKV, HD, max_pos, chunk)) return hipErrorInvalidValue;
+    for (int i = 0; i < 4; i++) form[i] = 0;
+    if (B == 0 || T == 0 || rows == 0) return hipSuccess;
+    const Kv8Plan pl = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window < 0 ? 0 : window, tree != 0);
+    form[0] = pl.tile;
+    form[1] = pl.tile ? pl.tile : 16 * pl.nt;
+    form[2] = pl.C;
+    form[3] = pl.ns;
+    return hipSuccess;
+}
+
 hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,
                         float *lse, int B, int T, int rows, int NQ, const int *ctx, const int *cu, const unsigned *anc, int max_pos,
                         int chunk, void *ws, size_t ws_bytes, hipStream_t st, float scale, int window) {
@@ -741,7 +753,7 @@ hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const 
         part.l = reinterpret_cast<float *>(static_cast<char *>(ws) + one);
         part.acc = reinterpret_cast<float *>(static_cast<char *>(ws) + 2 * one);
     }
-    const hipError_t e = timed_launch(st, [&] { return pl.prefill ? launch_kv8_prefill(p, part, st) : launch_kv8_decode(p, part, pl.nt, st); });
+    const hipError_t e = timed_launch(st, [&] { return pl.tile ? launch_kv8_prefill(p, part, pl, st) : launch_kv8_decode(p, part, pl, st); });
     if (e != hipSuccess || pl.ns == 1) return e;
     return launch_kv8_combine(p, part, st);
 }

@@ -112,14 +112,16 @@ hipError_t launch_kv8_append(const void *k, const void *v, int src_dtype, long k
 
 // Split-KV form: single tokens, short runs, trees, small prompts (any T; rows of a KV head in groups of 16 nt, nt 1, 2 or 4;
 // at HD 512 1 or 2).
-hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, int nt, hipStream_t st);
+struct Kv8Plan;
+hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st);
 // Prompt form: 64 or 128 rows of a KV head per workgroup, no tree masks.
-hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st);
+hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st);
 hipError_t launch_kv8_combine(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st);
 
-// What a call runs: the form, the split-KV form's row groups, the keys of a split (0: the prompt form's one pass) and how many
-// splits max_pos reaches (1: the kernel writes O, no workspace).
-struct Kv8Plan { bool prefill; int nt, C, ns; };
+// What a call runs: the rows of a prompt tile (0: the split-KV form, in groups of 16 nt rows), the keys of a split (0: the
+// prompt form's one pass), how many splits max_pos reaches (1: the kernel writes O, no workspace), and how many of them the
+// keys of one request's rows reach at most.
+struct Kv8Plan { int tile, nt, C, ns; long long per; };
 Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, bool tree);
 
 }  // namespace dgx

@@ -609,7 +609,7 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     long long keys = max_pos + 1ll;
     if (window > 0) keys = std::min<long long>(keys, (long long)window + T - 1);
     const int whole = (max_pos / 128 + 1) * 128;                       // a split that holds every key
-    Kv8Plan pl{false, 0, chunk, 1};
+    Kv8Plan pl{0, 0, chunk, 1, 1};
     if (tree || hr <= 64) {
         pl.nt = hr <= 16 ? 1 : hr <= 32 || HD == 512 ? 2 : 4;
         // Keys of a split, by the call's K and V in heads of 256 dims. Short ones leave a call to the prologues of its
@@ -630,8 +630,8 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
         // behind 2000 (250) 75.8 | 79.0; behind a window of 1024 500 x 16 over 8 (125) 35.2 | 38.2, 600 (150) 41.9 | 38.8; HD 512
         // 800 x 16 (200) 42.7 | 46.7, 1024 (256) 57.1 | 54.2.
         const long long n64 = std::min((long long)B * ((hr + 63) / 64), (long long)rows * G / 64 + B) * NKV;
-        pl.prefill = n64 >= (HD == 512 ? 250 : window > 0 && window <= max_pos ? 140 : keys <= 2304 ? 360 : 280);
-        if (!pl.prefill) {
+        pl.tile = n64 >= (HD == 512 ? 250 : window > 0 && window <= max_pos ? 140 : keys <= 2304 ? 360 : 280) ? 64 : 0;
+        if (!pl.tile) {
             // 200 x 16 q-heads over 8 without a prefix: groups of 16 rows 9.5 us, 32 12.2, 64 16.9; 1000 behind 1000: 72, 53 and
             // 64; 512 behind 4096: 64 rows in 1536-key splits 74, in 1024 87, no split of 16 rows 93. Fewer workgroups at HD
             // 512: 500 x 16 over 1 behind 4000 117 us unsplit, 138 in 1536; 100 behind 4000 41 in 1024, 52 in 512.
@@ -643,19 +643,26 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
                 const long long splits = std::max(1ll, (want + n / 2) / n);
                 pl.C = splits == 1 ? whole : (int)std::min(2048ll, std::max(512ll, (keys / splits + 127) / 128 * 128));
             }
-        } else if (chunk == 0) return pl;
+        }
     }
-    pl.ns = max_pos / pl.C + 1;
-    if (pl.prefill && pl.ns == 1) pl.C = 0;
+    if (pl.C) {
+        pl.ns = max_pos / pl.C + 1;
+        pl.per = window > 0 ? std::min<long long>(pl.ns, ((long long)window + T - 2) / pl.C + 2) : pl.ns;
+    }
+    if (!pl.tile) return pl;
+    if (pl.ns == 1) pl.C = 0;
+    // Tiles of 128 rows where there are two rounds of them for the 512 workgroups that run at once (one, under a window: its
+    // tiles are equally long), else of 64. HD 256, us of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400 tiles
+    // of 128) 326 | 361, 4096 behind a window of 1024, 16 over 8 (512) 79.7 | 87.9, causal 4096 of those (512) 202 | 153.
+    const long long all = std::min((long long)B * T, (long long)rows) * NQ * (pl.ns > 1 ? std::max(2ll, pl.per) : 1);
+    if (HD < 512 && all >= 128 * (window > 0 && window < max_pos ? 500 : 960)) pl.tile = 128;
     return pl;
 }
 
-hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, int nt, hipStream_t st) {
-    const int G = p.NQ / p.c.NKV, rows = (int)std::min<long long>((long long)p.T * G, INT_MAX);
+hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st) {
+    const int nt = pl.nt, G = p.NQ / p.c.NKV, rows = (int)std::min<long long>((long long)p.T * G, INT_MAX);
     Kv8DecArgs a{p, part, part.C, div_magic(part.C), (rows + 16 * nt - 1) / (16 * nt), 0, part.ns == 1, p.scale * kLog2e};
-    long long per = p.max_pos / part.C + 1;
-    if (p.window > 0) per = std::min<long long>(per, ((long long)p.window + p.T - 2) / part.C + 2);
-    const long long raw = per * p.B * p.c.NKV, units = a.nrg == 1 || raw < 64 ? raw : (raw + 7) / 8 * 8, wgs = units * a.nrg;
+    const long long raw = pl.per * p.B * p.c.NKV, units = a.nrg == 1 || raw < 64 ? raw : (raw + 7) / 8 * 8, wgs = units * a.nrg;
     if (a.nrg == 1 || raw < 64) a.spread = (int)raw;
     if (!kv8_grid_ok(wgs, p.c.HD == 512 && nt > 1 ? 512 : 256)) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)wgs);

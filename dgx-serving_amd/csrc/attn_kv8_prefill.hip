@@ -499,19 +499,9 @@ template <int HD, class Cf> static hipError_t launch_pre(const Kv8PrefArgs &a, h
     return a.p.q_dtype == DT_F16 ? launch_pre_k<HD, Cf, true>(a, st) : launch_pre_k<HD, Cf, false>(a, st);
 }
 
-hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st) {
-    Kv8PrefArgs a{p, part, part.C ? div_magic(part.C) : 0u, 1, p.scale * kLog2e};
-    const long long G = p.NQ / p.c.NKV;
-    if (part.C) {
-        long long per = p.max_pos / part.C + 1;
-        if (p.window > 0) per = std::min<long long>(per, ((long long)p.window + p.T - 2) / part.C + 2);
-        a.ns = (int)std::max(2ll, per);
-    }
-    // Tiles of 128 rows where there are two rounds of them for the 512 workgroups that run at once (one, under a window: its
-    // tiles are equally long), else of 64. HD 256, us of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400 tiles
-    // of 128) 326 | 361, 4096 behind a window of 1024, 16 over 8 (512) 79.7 | 87.9, causal 4096 of those (512) 202 | 153.
-    const long long rows = std::min((long long)p.B * p.T, (long long)p.rows) * G * p.c.NKV * a.ns;
-    const bool wide = rows >= 128 * (p.window > 0 && p.window < p.max_pos ? 500 : 960);
+hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st) {
+    const Kv8PrefArgs a{p, part, part.C ? div_magic(part.C) : 0u, part.C ? (int)std::max(2ll, pl.per) : 1, p.scale * kLog2e};
+    const bool wide = pl.tile == 128;
     switch (p.c.HD) {
     case 128: return wide ? launch_pre<128, Kv8PrefCfg<128, 2, 4, 1, 2, 2>>(a, st) : launch_pre<128, Kv8PrefCfg<128, 2, 2, 2, 1, 3>>(a, st);
     case 256: return wide ? launch_pre<256, Kv8PrefCfg<256, 2, 4, 1, 2, 2>>(a, st) : launch_pre<256, Kv8PrefCfg<256, 2, 2, 2, 1, 2>>(a, st);

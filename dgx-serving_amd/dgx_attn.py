@@ -59,6 +59,7 @@ def lib():
             "dgx_kv8_append": ([P, P, I, L64, L64, P, P, I, P], I),
             "dgx_attn_kv8": ([P, I, P, P, L64, P, I, P, I, I, I, I, P, P, P, I, I, P, S, P, F, I], I),
             "dgx_attn_kv8_workspace": ([I, I, I, I, I, I, I, I, I, I], S),
+            "dgx_attn_kv8_form": ([I, I, I, I, I, I, I, I, I, I, P], I),
             "dgx_attn_version": ([], ctypes.c_char_p),
             "dgx_attn_timing": ([I], I),
             "dgx_attn_timing_read": ([P, P], I),
@@ -351,6 +352,15 @@ def attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk=0, window=0, tree
     n = lib().dgx_attn_kv8_workspace(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, 1 if tree else 0)
     _need(n != ctypes.c_size_t(-1).value, "attn_kv8_workspace: sizes that dgx_attn_kv8 refuses")
     return n
+
+
+def attn_kv8_form(B, T, rows, NQ, NKV, HD, max_pos, chunk=0, window=0, tree=False):
+    """The form attn_kv8 takes for these sizes (dgx_attn_kv8_form): (tile rows or 0, rows of a workgroup, keys of a split or 0,
+    splits of a row)."""
+    form = (ctypes.c_int * 4)()
+    _need(lib().dgx_attn_kv8_form(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, 1 if tree else 0, form) == 0,
+          "attn_kv8_form: sizes that dgx_attn_kv8 refuses")
+    return tuple(form)
 
 
 def attn_kv8(Q, cache, table, ctx, O, T, max_pos, cu=None, anc=None, chunk=0, ws=None, scale=0.0, window=0, lse=None):

@@ -278,6 +278,10 @@ hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const 
 /* Bytes of ws for dgx_attn_kv8 with these sizes (others, smaller ones too, may take another form and need more). tree 1: for calls with anc; 0: for calls
  * without, and at T <= 32 for both. (size_t)-1 for sizes that the call refuses. */
 size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree);
+/* The form that dgx_attn_kv8 takes for these sizes (for tests, benchmarks and profilers; host only): form[0] the rows of a
+ * prompt tile, 64 or 128, or 0 for the split-KV form; form[1] the query rows of a workgroup; form[2] the keys of a split, 0 for
+ * prompts in one pass; form[3] the splits of a row in the workspace (1: none is used). All 0 where there is nothing to do. */
+hipError_t dgx_attn_kv8_form(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, int tree, int form[4]);
 
 /* Measurement hook (no counterpart in the reference; for benchmarks and profilers). With timing on, the main
  * kernel of every decode/verify (split or streaming kernel, without the LSE combine) and every prefill launch is

@@ -186,3 +186,57 @@ def blank_tail(K, V, table, lens, page, code=0x7F):
     p, o = np.nonzero(~used)
     K[p, :, o, :] = code
     V[p, :, :, o] = code
+
+
+def attention_rows(Q, K, V, Ks, Vs, table, ctx, cu, scale=0.0, window=0, anc=None):
+    """attention() for larger calls: the same values and the same bounds, a request and KV head at a time."""
+    rows_n, NQ, HD = Q.shape
+    P, NKV, page, _ = K.shape
+    G = NQ // NKV
+    sc = scale if scale > 0 else 1.0 / np.sqrt(HD)
+    O, lse, tol = np.full(Q.shape, np.nan), np.full((rows_n, NQ), np.nan), np.zeros(Q.shape)
+    lse_tol = np.zeros((rows_n, NQ))
+    for b in range(len(ctx)):
+        n0, n, r0 = int(ctx[b]), int(cu[b + 1] - cu[b]), int(cu[b])
+        if n <= 0:
+            continue
+        L = max(n0 + n, 0)
+        j, pos = np.arange(L), n0 + np.arange(n)
+        ids = np.asarray(table[b], np.int64)[j // page]
+        ok = (ids >= 0) & (ids < P)
+        ids, off = np.where(ok, ids, 0), j % page
+        att = ok & (j <= pos[:, None])
+        if window > 0:
+            att &= j > pos[:, None] - window
+        if anc is not None:
+            d = j - n0
+            att &= (d < 0) | ((np.asarray(anc[r0:r0 + n], np.int64)[:, None] >> np.clip(d, 0, 31)) & 1).astype(bool)
+        some, att = att.any(0), np.repeat(att, G, 0)                   # rows: token-major, then q-heads
+        nk, empty = att.sum(1), ~att.any(1)
+        for h in range(NKV):
+            q = Q[r0:r0 + n, h * G:(h + 1) * G].reshape(n * G, HD)
+            k = np.where(some[:, None], TABLE[K[ids, h, off]] * Ks[ids, h].astype(np.float64)[:, None], 0.0)
+            v = np.where(some[:, None], TABLE[V[ids, h, :, off]] * Vs[ids, h].astype(np.float64)[:, None], 0.0)
+            s = np.where(att, (q @ k.T) * sc, -np.inf)
+            top = np.where(empty, 0.0, s.max(1, initial=-np.inf))
+            w = np.exp(s - top[:, None])
+            l = w.sum(1)
+            w /= np.where(empty, 1.0, l)[:, None]
+            ds = np.where(att, HD * 2.0 ** -24 * (np.abs(q) @ np.abs(k).T) * sc + 2.0 ** -22 * np.abs(s), 0.0).max(1, initial=0.0) + 2.0 ** -21
+            vmax = np.where(att, np.abs(v).max(1, initial=0.0), 0.0).max(1, initial=0.0)
+            rel = 2.0 ** -11 + 2 * ds + 2 * nk * 2.0 ** -24
+            at = (slice(r0, r0 + n), slice(h * G, (h + 1) * G))
+            with np.errstate(divide="ignore"):
+                L1 = np.where(empty, -np.inf, top + np.log(l))
+            O[at], lse[at] = (w @ v).reshape(n, G, HD), L1.reshape(n, G)
+            tol[at] = (rel[:, None] * (w @ np.abs(v)) + (nk * 2.0 ** -30 * vmax)[:, None]).reshape(n, G, HD)
+            lse_tol[at] = np.where(empty, 0.0, ds + nk * 2.0 ** -24 + 2.0 ** -22 * np.abs(np.where(empty, 0.0, L1)) + 2.0 ** -20).reshape(n, G)
+    return O, lse, tol, lse_tol
+
+
+def make_cache_fast(rng, P, page, NKV, HD, spread=2):
+    """make_cache() with values drawn from 2^16 normal ones."""
+    pool = encode(rng.standard_normal(1 << 16) * 60)
+    K, V = (pool[rng.integers(0, 1 << 16, s)] for s in ((P, NKV, page, HD), (P, NKV, HD, page)))
+    Ks, Vs = (2.0 ** (rng.integers(0, spread + 1, (P, NKV)) - 6.0) for _ in range(2))
+    return K, V, Ks.astype(np.float32), Vs.astype(np.float32)
