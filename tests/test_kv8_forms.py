@@ -19,9 +19,9 @@ def test_the_form_of_refused_sizes_is_refused(kw):
 
 
 def test_the_calls_of_the_gpu_tests_take_their_forms():
-    """Every prompt tile, in one pass and in splits."""
+    """Every prompt tile, in one pass and in splits, and the split-KV form beside them."""
     seen = set()
-    for heads, page, io, ctx, add, window, chunk, tile, split in G.CALLS.values():
+    for heads, page, io, ctx, add, window, chunk, tile, split in [*G.CALLS.values(), *G.SMALL.values()]:
         f = G.form_of(heads, ctx, add, sum(add) + 3, window, chunk)
         assert f[0] == tile and (f[3] > 1) == split and f[1] in ((tile,) if tile else (16, 32, 64)), f
         seen.add((heads[2], f[0], f[3] > 1, window > 0))

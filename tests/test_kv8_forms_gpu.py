@@ -166,6 +166,49 @@ def raw(seed, heads, page, io, ctx, add, window, chunk, change_q):
     return O
 
 
+# Rows that attend pages of small scales only, beside rows of large ones: 2^40 between them, so nothing of the large ones may
+# reach their sums, and the bound is that of the small values.
+SMALL = {
+    "single tokens": ((12, 2, 256), 16, "f16", [100, 90, 130], [1, 1, 1], 0, 0, 0, False),
+    "single tokens in splits": ((8, 2, 128), 16, "bf16", [200, 190, 230], [1, 1, 1], 0, 64, 0, True),
+    "short runs in a window": ((4, 2, 128), 16, "f16", [40, 90], [32, 32], 8, 0, 0, False),
+    "short runs in a window, splits": ((16, 1, 512), 16, "f16", [40, 90], [8, 8], 8, 64, 0, True),
+    "prompts in groups of rows": ((8, 2, 256), 16, "bf16", [0, 90], [90, 70], 8, 0, 0, False),
+    "64-row tiles": ((96, 48, 128), 16, "f16", [0, 90], [90, 70], 8, 0, 64, False),
+    "64-row tiles, HD 512": ((64, 64, 512), 16, "bf16", [40, 0, 200], [130, 90, 70], 8, 0, 64, False),
+    "64-row tiles in splits": ((64, 32, 256), 16, "f16", [120, 0, 40], [90, 65, 80], 8, 64, 64, True),
+    "128-row tiles": ((384, 64, 128), 16, "f16", [150, 0], [99, 90], 8, 0, 128, False),
+    "128-row tiles in splits": ((192, 32, 256), 16, "bf16", [200, 0, 70], [130, 110, 129], 8, 64, 128, True),
+}
+
+
+@pytest.mark.parametrize("name", SMALL)
+def test_small_scales_beside_large_ones(name):
+    heads, page, io, ctx, add, window, chunk, tile, split = SMALL[name]
+    small = np.float32(2.0 ** -30)
+
+    def hurt(K, V, Ks, Vs, table):
+        Ks[:] = 2.0 ** -8
+        Vs[:] = 2.0 ** 10
+        if window:                                                   # every other page: windows of 8 keys lie in one or two
+            for b in range(len(ctx)):
+                ids = table[b, ::2]
+                Vs[ids[ids >= 0]] = small
+        else:                                                        # every other request
+            for b in range(0, len(ctx), 2):
+                Vs[table[b][table[b] >= 0]] = small
+    O, lse, cu = call(7, heads, page, io, ctx, add, tile, split, window=window, chunk=chunk, hurt=hurt, out="fp32")
+    pos = np.concatenate([c + np.arange(a) for c, a in zip(ctx, add)])
+    if window:
+        # every key of the window in one page of an even column
+        only = torch.from_numpy((pos // page == np.maximum(pos - window + 1, 0) // page) & (pos // page % 2 == 0))
+    else:
+        only = torch.from_numpy(np.repeat(np.arange(len(ctx)) % 2 == 0, add))
+    top = O[:int(cu[-1])].abs().amax(dim=(1, 2)).cpu()
+    assert int(only.sum()) > 1 and bool((top[only] <= 448 * float(small)).all()) and bool((top[only] > float(small)).all())
+    assert bool((top[~only] > 1e-3).all())
+
+
 def test_captured_tiles_in_splits():
     """128-row tiles in key splits, captured at the largest sizes and replayed on other lengths, against the same call made eagerly."""
     heads, page, io, ctx, add, window, chunk, tile, split = CALLS["128 in splits, HD 256, window"]
@@ -198,3 +241,23 @@ def test_captured_tiles_in_splits():
         ref = R.attention_rows(Q.double().cpu().numpy(), K, V, Ks, Vs, table.cpu().numpy(), lens, np.concatenate([[0], np.cumsum(news)]), window=window)
         R.check(O, None, ref, str(lens))
         assert bool((O[n:] == 2).all())
+
+
+@pytest.mark.parametrize("heads,add", [((24, 4, 256), [8, 5, 1]), ((16, 1, 512), [4, 4, 2]), ((8, 2, 128), [32, 17, 9])])
+@pytest.mark.parametrize("window,chunk", [(5, 0), (40, 64), (200, 128)])
+def test_trees_behind_a_window(heads, add, window, chunk):
+    """Ancestor masks and a window together: tokens of the window that the tree leaves."""
+    NQ, NKV, HD = heads
+    rng = np.random.default_rng(9)
+    page, ctx = 16, np.array([0, 70, 300])
+    add = np.array(add)
+    lens, cu = ctx + add, np.concatenate([[0], np.cumsum(add)])
+    P, rows = int((-(-lens // page)).sum()), int(cu[-1])
+    table = R.tables(rng, lens, page, P)
+    K, V, Ks, Vs = R.make_cache_fast(rng, P, page, NKV, HD)
+    anc = rng.integers(0, 1 << 32, rows).astype(np.uint32)
+    Q = torch.from_numpy(rng.standard_normal((rows, NQ, HD))).half()
+    O, lse = torch.empty(rows, NQ, HD, device="cuda").half(), torch.empty(rows, NQ, device="cuda")
+    A.attn_kv8(Q.cuda(), R.to_cache(A, K, V, Ks, Vs), i32(table), i32(ctx), O, int(add.max()), int(lens.max()) - 1, cu=i32(cu),
+               anc=torch.from_numpy(anc.view(np.int32)).cuda(), chunk=chunk, window=window, lse=lse)
+    R.check(O, lse, R.attention_rows(Q.double().numpy(), K, V, Ks, Vs, table, ctx, cu, window=window, anc=anc), f"{heads}")
