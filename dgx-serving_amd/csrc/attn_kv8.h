@@ -12,6 +12,7 @@
 #pragma once
 #include "attn_device.h"
 #include "attn_internal.h"
+#include <climits>
 
 namespace dgx {
 
@@ -77,11 +78,16 @@ __device__ __forceinline__ void kv8_rows(const Kv8Problem &p, int b, int &r0, in
     }
 }
 
+// Position of request b's first row, which leaves its n rows below INT_MAX.
+__device__ __forceinline__ int kv8_first_pos(const Kv8Problem &p, int b, int n) { return min(p.ctx[b], INT_MAX - n); }
+
 // Partials of a split call: index (r * NQ + head) * ns + split; acc[HD], reference exponent m and sum l: the row's output is
-// sum acc 2^(m - M) / sum l 2^(m - M) over the splits, M the largest m.
+// sum acc 2^(m - M) / sum l 2^(m - M) over the splits, M the largest m. Splits lie at absolute keys c C .., but are counted from
+// the one with the first key of the request's first row: behind a window the room that a row needs does not grow with the
+// positions (16 drafts of 8 tokens, 16 q-heads over 8 of 256, window 1024, max_pos 131071: 13 MB, counted from key 0 1082).
 struct Kv8Partials {
     float *m, *l, *acc;
-    int ns, C;                        // splits of a row at most, keys of a split (0: none, the kernel writes O itself)
+    int ns, C;                        // splits that a row has room for, keys of a split (0: none, the kernel writes O itself)
 };
 
 // A value that is the same in all lanes and that no kernel of this library writes while this one runs, through the scalar
@@ -119,9 +125,9 @@ hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, cons
 hipError_t launch_kv8_combine(const Kv8Problem &p, const Kv8Partials &part, hipStream_t st);
 
 // What a call runs: the rows of a prompt tile (0: the split-KV form, in groups of 16 nt rows), the keys of a split (0: the
-// prompt form's one pass), how many splits max_pos reaches (1: the kernel writes O, no workspace), and how many of them the
-// keys of one request's rows reach at most.
-struct Kv8Plan { int tile, nt, C, ns; long long per; };
+// prompt form's one pass) and how many splits the keys of one request's rows reach at most (1: the kernel writes O, no
+// workspace).
+struct Kv8Plan { int tile, nt, C, ns; };
 Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos, int chunk, int window, bool tree);
 
 }  // namespace dgx

@@ -41,10 +41,10 @@ struct Kv8DecArgs {
     float sl2;                        // scale * log2(e)
 };
 
-// Work item `rest` -> request, chunk and the keys [lo, hi) of the request's rows; the shorter of a request's first and
-// last chunk come behind all others (the scheme and its reasons are find_item's).
+// Work item `rest` -> request, its first chunk, the item's chunk and the keys [lo, hi) of the request's rows; the shorter of a
+// request's first and last chunk come behind all others (the scheme and its reasons are find_item's).
 // With `all`, a request whose rows have no key at all is an item too (its rows are written in the kernel).
-__device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M, bool all, int rest, int &seq, int &c, int &lo, int &hi) {
+__device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M, bool all, int rest, int &seq, int &c_first, int &c, int &lo, int &hi) {
     const int lane = threadIdx.x & 63;
     for (int phase = 0; phase < 2; phase++)
         for (int s0 = 0; s0 < p.B; s0 += 64) {
@@ -52,7 +52,7 @@ __device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M,
             if (s0 + lane < p.B) {
                 int r0, nr;
                 kv8_rows(p, s0 + lane, r0, nr);
-                const int p0 = p.ctx[s0 + lane], pl = min(p0, INT_MAX - nr) + nr - 1;
+                const int p0 = kv8_first_pos(p, s0 + lane, nr), pl = p0 + nr - 1;
                 lo_s = win_lo(p0, p.window); hi_s = nr > 0 ? min(pl, p.max_pos) + 1 : 0;
                 first = div_by(lo_s, C, M);
                 n = hi_s > lo_s ? div_by(hi_s - 1, C, M) - first + 1 : all && nr > 0 ? 1 : 0;
@@ -65,7 +65,7 @@ __device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M,
                 const int l = __builtin_ctzll(hit), r = rest - (incl - m);
                 const int cc = first + (phase == 1 ? sh : r < sh ? r : r + 1);
                 seq = s0 + l;
-                c = __builtin_amdgcn_readlane(cc, l); lo = __builtin_amdgcn_readlane(lo_s, l); hi = __builtin_amdgcn_readlane(hi_s, l);
+                c_first = __builtin_amdgcn_readlane(first, l); c = __builtin_amdgcn_readlane(cc, l); lo = __builtin_amdgcn_readlane(lo_s, l); hi = __builtin_amdgcn_readlane(hi_s, l);
                 return true;
             }
             rest -= __builtin_amdgcn_readlane(incl, 63);
@@ -108,9 +108,10 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     int unit, rg;
     if (a.spread) { rg = a.nrg - 1 - (int)blockIdx.x / a.spread; unit = (int)blockIdx.x % a.spread; }
     else { unit = (int)(blockIdx.x / (8 * a.nrg)) * 8 + (int)(blockIdx.x & 7); rg = a.nrg - 1 - (int)(blockIdx.x >> 3) % a.nrg; }
-    int seq, c, lo, hi;
-    if (!kv8_find(p, a.C, a.Cm, a.direct, unit / kc.NKV, seq, c, lo, hi)) return;
+    int seq, c_first, c, lo, hi;
+    if (!kv8_find(p, a.C, a.Cm, a.direct, unit / kc.NKV, seq, c_first, c, lo, hi)) return;
     seq = __builtin_amdgcn_readfirstlane(seq); c = __builtin_amdgcn_readfirstlane(c);
+    const int place = __builtin_amdgcn_readfirstlane(c - c_first);     // of the chunk among the request's
     lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi);
     const int h = unit % kc.NKV, G = p.NQ / kc.NKV;
     int row0, nr;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
     const int rho0 = rg * Cf::RR, nrows = min(nr * G - rho0, Cf::RR);
     if (nrows <= 0) return;
     // Keys of the chunk that some row of this group attends.
-    const int p0 = min(scalar_load(p.ctx + seq), INT_MAX - nr), t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
+    const int p0 = min(scalar_load(p.ctx + seq), INT_MAX - nr) /* kv8_first_pos */, t_a = rho0 / G, t_b = (rho0 + nrows - 1) / G;
     const int j_lo = max(c * a.C, win_lo(p0 + t_a, p.window)), j_hi = min(min(hi, p0 + t_b + 1) - c * a.C, a.C) + c * a.C;
     if (j_lo >= j_hi && !a.direct) return;
 
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__((Kv8DecCfg<HD, NT>::NW * 64), (Kv8DecCfg<HD, N
             for (int d = 0; d < DB; d++) kv8_store4(p, row * HD + dim0 + 16 * d, acc[nt][d] * inv);
             if (wave == 0 && g == 0 && p.lse) p.lse[row] = L == 0.f ? kNegInf : (m[nt] + __builtin_amdgcn_logf(L)) * kLn2;
         } else {
-            const size_t x = row * a.part.ns + c;
+            const size_t x = row * a.part.ns + place;
 #pragma unroll
             for (int d = 0; d < DB; d++) *reinterpret_cast<f32x4 *>(a.part.acc + x * HD + dim0 + 16 * d) = acc[nt][d];
             if (wave == 0 && g == 0) { a.part.m[x] = m[nt]; a.part.l[x] = L; }
@@ -443,8 +444,8 @@ struct Kv8CombArgs {
     int by_row;                       // items are rows of the buffers, not the T rows that each request has at most
 };
 
-// The splits [c0, c0 + n) of item bt's row, and the row's first element among the partials; false past the last row. All lanes
-// of a wave ask for the same item.
+// The places [c0, c0 + n) of the splits of item bt's row among its request's, and the row's place among the partials' rows;
+// false past the last row. All lanes of a wave ask for the same item.
 __device__ __forceinline__ bool comb_row(const Kv8CombArgs &a, int bt, int head, size_t &row, int &c0, int &n) {
     const Kv8Problem &p = a.p;
     int b, i, row0, nr;
@@ -460,10 +461,11 @@ __device__ __forceinline__ bool comb_row(const Kv8CombArgs &a, int bt, int head,
         kv8_rows(p, b, row0, nr);
     }
     if ((unsigned)i >= (unsigned)nr) return false;
-    const int pos = min(p.ctx[b], INT_MAX - i) + i, lo = win_lo(pos, p.window), hi = min(pos, p.max_pos);
+    const int p0 = kv8_first_pos(p, b, nr), pos = p0 + i, lo = win_lo(pos, p.window), hi = min(pos, p.max_pos);
+    const int c_lo = div_by(lo, a.part.C, a.Cm);
     row = (size_t)(row0 + i) * p.NQ + head;
-    c0 = div_by(lo, a.part.C, a.Cm);
-    n = hi >= lo ? div_by(hi, a.part.C, a.Cm) - c0 + 1 : 0;
+    c0 = c_lo - div_by(win_lo(p0, p.window), a.part.C, a.Cm);
+    n = hi >= lo ? div_by(hi, a.part.C, a.Cm) - c_lo + 1 : 0;
     return true;
 }
 
@@ -609,7 +611,7 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     long long keys = max_pos + 1ll;
     if (window > 0) keys = std::min<long long>(keys, (long long)window + T - 1);
     const int whole = (max_pos / 128 + 1) * 128;                       // a split that holds every key
-    Kv8Plan pl{0, 0, chunk, 1, 1};
+    Kv8Plan pl{0, 0, chunk, 1};
     if (tree || hr <= 64) {
         pl.nt = hr <= 16 ? 1 : hr <= 32 || HD == 512 ? 2 : 4;
         // Keys of a split, by the call's K and V in heads of 256 dims. Short ones leave a call to the prologues of its
@@ -647,14 +649,16 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     }
     if (pl.C) {
         pl.ns = max_pos / pl.C + 1;
-        pl.per = window > 0 ? std::min<long long>(pl.ns, ((long long)window + T - 2) / pl.C + 2) : pl.ns;
+        // The keys of a request's rows behind a window are window + T - 1 neighbours. (Where max_pos reaches a second split there
+        // are two places at least: the form with one has no bounds but a request's own.)
+        if (window > 0 && pl.ns > 2) pl.ns = (int)std::min<long long>(pl.ns, std::max(2ll, ((long long)window + T + pl.C - 3) / pl.C + 1));
     }
     if (!pl.tile) return pl;
     if (pl.ns == 1) pl.C = 0;
     // Tiles of 128 rows where there are two rounds of them for the 512 workgroups that run at once (one, under a window: its
     // tiles are equally long), else of 64. HD 256, us of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400 tiles
     // of 128) 326 | 361, 4096 behind a window of 1024, 16 over 8 (512) 79.7 | 87.9, causal 4096 of those (512) 202 | 153.
-    const long long all = std::min((long long)B * T, (long long)rows) * NQ * (pl.ns > 1 ? std::max(2ll, pl.per) : 1);
+    const long long all = std::min((long long)B * T, (long long)rows) * NQ * pl.ns;
     if (HD < 512 && all >= 128 * (window > 0 && window < max_pos ? 500 : 960)) pl.tile = 128;
     return pl;
 }
@@ -662,7 +666,7 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
 hipError_t launch_kv8_decode(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st) {
     const int nt = pl.nt, G = p.NQ / p.c.NKV, rows = (int)std::min<long long>((long long)p.T * G, INT_MAX);
     Kv8DecArgs a{p, part, part.C, div_magic(part.C), (rows + 16 * nt - 1) / (16 * nt), 0, part.ns == 1, p.scale * kLog2e};
-    const long long raw = pl.per * p.B * p.c.NKV, units = a.nrg == 1 || raw < 64 ? raw : (raw + 7) / 8 * 8, wgs = units * a.nrg;
+    const long long raw = (long long)pl.ns * p.B * p.c.NKV, units = a.nrg == 1 || raw < 64 ? raw : (raw + 7) / 8 * 8, wgs = units * a.nrg;
     if (a.nrg == 1 || raw < 64) a.spread = (int)raw;
     if (!kv8_grid_ok(wgs, p.c.HD == 512 && nt > 1 ? 512 : 256)) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)wgs);

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(Cf::NW * 64, Cf::OCC) kv8_prefill_kernel(const
     int row0, nr;
     kv8_rows(p, seq, row0, nr);
     row0 = __builtin_amdgcn_readfirstlane(row0); nr = __builtin_amdgcn_readfirstlane(nr);
-    const int p0 = min(scalar_load(p.ctx + seq), INT_MAX - nr);
+    const int p0 = min(scalar_load(p.ctx + seq), INT_MAX - nr);          // (kv8_first_pos)
     const int rho0 = tile * Cf::RR, nrows = min(nr * G - rho0, Cf::RR);
     const int tok_a = rho0 / G, tok_b = (rho0 + nrows - 1) / G;        // first and last token of the tile
     int j_lo = win_lo(p0 + tok_a, p.window), j_hi = min(p0 + tok_b, p.max_pos) + 1;
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(Cf::NW * 64, Cf::OCC) kv8_prefill_kernel(const
         const size_t row = (size_t)(row0 + rho / G) * p.NQ + h * G + rho % G;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const int dim = kg * DK * 16 + 4 * g;
-        const size_t px = row * a.part.ns + (a.ns > 1 ? div_by(j_lo, a.part.C, a.Cm) : 0);
+        const size_t px = row * a.part.ns + (a.ns > 1 ? div_by(j_lo, a.part.C, a.Cm) - div_by(win_lo(p0, p.window), a.part.C, a.Cm) : 0);
 #pragma unroll
         for (int d = 0; d < DK; d++) {
             f32x4 v = acc[rb][d];
@@ -500,7 +500,7 @@ template <int HD, class Cf> static hipError_t launch_pre(const Kv8PrefArgs &a, h
 }
 
 hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st) {
-    const Kv8PrefArgs a{p, part, part.C ? div_magic(part.C) : 0u, part.C ? (int)std::max(2ll, pl.per) : 1, p.scale * kLog2e};
+    const Kv8PrefArgs a{p, part, part.C ? div_magic(part.C) : 0u, pl.ns, p.scale * kLog2e};
     const bool wide = pl.tile == 128;
     switch (p.c.HD) {
     case 128: return wide ? launch_pre<128, Kv8PrefCfg<128, 2, 4, 1, 2, 2>>(a, st) : launch_pre<128, Kv8PrefCfg<128, 2, 2, 2, 1, 3>>(a, st);

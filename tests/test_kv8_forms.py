@@ -1,6 +1,7 @@
 """CPU checks of the query for the form that a call over the paged 8-bit cache takes."""
 import ctypes
 
+import numpy as np
 import pytest
 
 import dgx_attn as A
@@ -45,3 +46,20 @@ def test_a_workspace_is_wanted_where_the_form_has_splits():
                                 assert n >= B * T * NQ * form[3] * (HD + 2) * 4
                             elif T > 32:
                                 assert n == 0
+
+
+@pytest.mark.parametrize("window", [1, 2, 64, 1000, 4096])
+def test_the_workspace_of_a_window_does_not_grow_with_the_positions(window):
+    """Behind a window a row needs places for the splits of its request's keys alone: window + T - 1 neighbours."""
+    for B, T, NQ, NKV, HD in ((16, 1, 16, 8, 256), (16, 8, 16, 8, 256), (64, 1, 24, 4, 256), (1, 500, 16, 8, 256), (3, 32, 16, 1, 512), (2, 3000, 8, 2, 128)):
+        for chunk in (0, 64, 1024):
+            for tree in (False, True)[:1 + (T <= 32)]:
+                args = (B, T, B * T, NQ, NKV, HD)
+                size = {A.attn_kv8_workspace(*args, mp, chunk, window, tree) for mp in (window + T + 40000, 131071, (1 << 30) - 1)}
+                assert len(size) == 1
+                C, ns = A.attn_kv8_form(*args, 131071, chunk, window, tree)[2:]
+                if C:
+                    lo = np.arange(min(C, 131072))                    # every place of the first key in its split
+                    most = ((lo + window + T - 2) // C - lo // C + 1).max()
+                    assert ns == min(131071 // C + 1, max(2, most)), (C, ns, most)
+    assert A.attn_kv8_workspace(16, 8, 128, 16, 8, 256, 131071, window=1024) < 1 << 24

@@ -261,3 +261,42 @@ def test_trees_behind_a_window(heads, add, window, chunk):
     A.attn_kv8(Q.cuda(), R.to_cache(A, K, V, Ks, Vs), i32(table), i32(ctx), O, int(add.max()), int(lens.max()) - 1, cu=i32(cu),
                anc=torch.from_numpy(anc.view(np.int32)).cuda(), chunk=chunk, window=window, lse=lse)
     R.check(O, lse, R.attention_rows(Q.double().numpy(), K, V, Ks, Vs, table, ctx, cu, window=window, anc=anc), f"{heads}")
+
+
+@pytest.mark.parametrize("heads,page,add,window,chunk,tile", [
+    ((24, 4, 256), 64, [1, 1, 1, 1], 1000, 0, 0), ((16, 8, 256), 16, [1, 1, 1, 1], 65, 64, 0), ((16, 8, 256), 16, [1, 1, 1], 66, 64, 0),
+    ((16, 1, 512), 32, [8, 3, 1, 8], 700, 0, 0), ((8, 2, 128), 16, [32, 9, 1, 0], 1, 64, 0), ((8, 2, 128), 16, [32, 32, 20, 5], 2, 64, 0),
+    ((16, 4, 128), 16, [13, 8, 16], 128, 128, 0), ((12, 2, 256), 64, [90, 3, 77], 130, 64, 0), ((4, 2, 256), 32, [300], 600, 0, 0),
+    ((64, 32, 128), 64, [90, 65, 80], 70, 64, 64), ((128, 64, 512), 64, [66, 90], 129, 128, 64), ((192, 64, 256), 64, [130, 90], 64, 64, 128)])
+def test_splits_behind_a_window_far_from_the_first_key(heads, page, add, window, chunk, tile):
+    """Positions around 10^5 and 10^7, of which only the pages that the window reaches exist, in a workspace of exactly the size
+    that is asked for: results, and bytes behind the workspace."""
+    NQ, NKV, HD = heads
+    rng = np.random.default_rng(window + HD)
+    add = np.array(add)
+    B, T = len(add), int(add.max())
+    cu = np.concatenate([[0], np.cumsum(add)])
+    rows = int(cu[-1])
+    near = rng.integers(window + 64, window + 400, B)                # positions within the pages that exist
+    near[0] = -(-(window + 100) // 128) * 128 + window - 2            # first key one before a split's border
+    lens = near + add
+    P = int((-(-lens // page)).sum())
+    table = R.tables(rng, lens, page, P)
+    K, V, Ks, Vs = R.make_cache_fast(rng, P, page, NKV, HD)
+    R.blank_tail(K, V, table, lens, page)
+    Q = torch.from_numpy(rng.standard_normal((rows, NQ, HD))).half()
+    for shift in (0, 102400, 1 << 24):                                # multiples of every page and of the splits below
+        mp = int(lens.max()) - 1 + shift
+        form = A.attn_kv8_form(B, T, rows, NQ, NKV, HD, mp, chunk, window)
+        assert form[0] == tile and (form[3] > 1 or chunk == 0), form
+        n = A.attn_kv8_workspace(B, T, rows, NQ, NKV, HD, mp, chunk, window)
+        ws = torch.full((n + 4096,), 0xFF, dtype=torch.uint8, device="cuda")
+        t = np.full((B, mp // page + 1), -1, np.int32)
+        t[:, shift // page:] = table[:, :t.shape[1] - shift // page]
+        O, lse = torch.full((rows, NQ, HD), 77.0, dtype=torch.float16, device="cuda"), torch.empty(rows, NQ, device="cuda")
+        A.attn_kv8(Q.cuda(), R.to_cache(A, K, V, Ks, Vs), i32(t), i32(near + shift), O, T, mp, cu=i32(cu), chunk=chunk, window=window, lse=lse,
+                   ws=ws[:n])
+        torch.cuda.synchronize()
+        assert bool((ws[n:] == 0xFF).all()), "bytes behind the workspace were written"
+        ref = R.attention_rows(Q.double().numpy(), K, V, Ks, Vs, table, near, cu, window=window)
+        R.check(O, lse, ref, f"shift {shift}")
