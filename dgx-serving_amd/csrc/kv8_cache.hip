@@ -143,7 +143,7 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
                            const int *free_pages, int free_cap, const int *free_in, int *free_out, int *cu, int *slots, int rows,
                            int *status, hipStream_t st) {
     const PlanArgs a{ctx, add, free_pages, free_in, table, free_out, cu, slots, status, table_stride, B, lp, cols, rows, free_cap};
-    const int grid = free_in == free_out || rows <= 2048 ? 1 : std::min(128, (rows + 2047) / 2048);
+    const int grid = free_in == free_out || rows <= 2048 ? 1 : (int)std::min(128ll, (rows + 2047ll) / 2048);
     const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;     // fewer waves meet sooner at the barriers (4.5 us a call, 5.1 with 1024)
     if (rows <= kNarrow && cols <= kNarrow) hipLaunchKernelGGL(kv8_plan_kernel<int>, dim3(grid), dim3(threads), 0, st, a);
     else hipLaunchKernelGGL(kv8_plan_kernel<long long>, dim3(grid), dim3(threads), 0, st, a);
