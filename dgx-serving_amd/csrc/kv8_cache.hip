@@ -13,11 +13,11 @@ namespace dgx {
 // All or nothing: a step that needs more free pages, columns or rows than there are, or has a negative length, takes nothing
 // (status tells which), gives every row slot -1 and every request no rows.
 //
-// Bound by latency: lengths, scan, free ids, slots (256 requests of one token 3.1 us, 96 prompts of 123K rows in all 5.9). The
+// Bound by latency: lengths, scan, free ids, slots (256 requests of one token 3.1 us, 96 prompts of 109K rows in all 5.9). The
 // scans take one workgroup's time whatever the grid, so every workgroup does them (lengths come from the L2) and takes its
-// share of the rows, from 2048 each on: 96 prompts 98 us in one workgroup. A second launch behind a one-workgroup scan would
-// cost more than the scan. One workgroup alone does it all where the free count is updated in place (another workgroup
-// could read it late).
+// share of the rows, from 2048 each on: the 96 prompts take 97 us a call in one workgroup and 8 in 54. A second launch behind a
+// one-workgroup scan would cost more than the scan. One workgroup alone does it all where the free count is updated in place
+// (another workgroup could read it late).
 struct PlanArgs {
     const int *ctx, *add, *free_pages, *free_in;
     int *table, *free_out, *cu, *slots, *status;

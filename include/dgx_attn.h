@@ -237,7 +237,9 @@ typedef struct dgx_kv8 {
  * >= 0). It keeps its ceil(ctx / page) pages and takes what it needs besides from the top of the stack free_pages
  * [free_cap], whose count is free_in[0], in the order of the requests. Written: the new pages' entries of table, cu[B + 1]
  * (first row of each request among the step's rows), slots[rows] (page id * page + token of each row; -1 behind the last),
- * free_out[0] (the count left; may be free_in). The ids in the stack stay as they are.
+ * free_out[0] (the count left). The ids in the stack stay as they are. free_out may be free_in, but then one workgroup does
+ * the whole step: no matter up to 2048 rows, 97 us instead of 8 for 96 prompts of 109K tokens in all. Two counters that take turns
+ * keep the fast form.
  * status[0] = 0, or a sum of 1: too few free pages, 2: a request needs more than table_cols pages, 4: more than `rows` new
  * tokens, 8: a negative length or a count outside [0, free_cap]. Then the step takes nothing: table and count stay as they
  * are, every slot is -1 and cu is zero (an append and an attention call over them do nothing).
