@@ -286,7 +286,7 @@ def _table(t, dev, B, what):
 
 def _here(dev, what):
     """`dev` is the current device, whose stream the call takes."""
-    if dev < 0 or dev != _get_device():
+    if dev < 0 or dev != (torch.cuda.current_device() if _get_device is None else _get_device()):
         raise ValueError(f"{what}: the tensors are on {'the host' if dev < 0 else f'device {dev}'}, not on the current device")
 
 

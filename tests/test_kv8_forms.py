@@ -63,3 +63,13 @@ def test_the_workspace_of_a_window_does_not_grow_with_the_positions(window):
                     most = ((lo + window + T - 2) // C - lo // C + 1).max()
                     assert ns == min(131071 // C + 1, max(2, most)), (C, ns, most)
     assert A.attn_kv8_workspace(16, 8, 128, 16, 8, 256, 131071, window=1024) < 1 << 24
+
+
+def test_the_device_check_without_the_raw_getter(monkeypatch):
+    """A torch without the raw device getter: the checks ask torch.cuda, as the stream lookup does."""
+    monkeypatch.setattr(A, "_get_device", None)
+    monkeypatch.setattr(A.torch.cuda, "current_device", lambda: 1)
+    A._here(1, "attn_kv8")
+    for dev in (0, -1):
+        with pytest.raises(ValueError):
+            A._here(dev, "attn_kv8")
