@@ -22,8 +22,10 @@
 // Chunks and steps lie at absolute keys and a step's wave depends on its position alone: a row's bits do not depend on the
 // other requests of the batch.
 //
-// What bounds it: HBM bytes of K and V. Conversions (v_cvt_scalef32_pk_f16_fp8 issues at full rate: 4.7 cycles measured, as
-// an fma) and MFMAs take about a tenth of their pipes' time at 6 TB/s.
+// What bounds it: HBM bytes of K and V, where a call has enough of them (16 requests of 32K keys 5.8 TB/s, 16 of up to 8K 5.0
+// without the merge; a kernel that does nothing but read reaches 7.1 here); the steps of the longest workgroup where it has not.
+// Conversions (v_cvt_scalef32_pk_f16_fp8 issues at full rate: 4.7 cycles measured, as an fma) and MFMAs take about a tenth of
+// their pipes' time at 6 TB/s.
 #include "attn_kv8.h"
 #include <algorithm>
 #include <climits>
@@ -76,7 +78,9 @@ __device__ __forceinline__ bool kv8_find(const Kv8Problem &p, int C, uint32_t M,
 template <int HD, int NT>
 struct Kv8DecCfg {
     static constexpr int SK = 128;                     // keys of a step
-    static constexpr int NW = HD == 512 && NT > 1 ? 8 : 4;   // waves (8: registers)
+    // Waves. 8 where 4 would not hold the accumulators. (HD 512 with one row group fits 244 registers of 4 waves; 8 take 158 of
+    // them. 8 requests of up to 32K in five draws, geometric mean of the 512-key splits: 30.1 us in 4 waves, 27.8 in 8.)
+    static constexpr int NW = HD == 512 && NT > 1 ? 8 : 4;
     static constexpr int KT = SK / 16 / NW;            // 16-key tiles of a wave
     static constexpr int RR = 16 * NT;                 // query rows
     static constexpr int DC = HD / 64;                 // 64-dim pieces of a key (one 16-byte load per lane each)
@@ -89,7 +93,9 @@ struct Kv8DecCfg {
     static constexpr size_t LDS_Q = (size_t)RR * QSTR * 2, LDS_P = (size_t)RR * PSTR * 2, LDS_K = KLDS ? (size_t)NW * 16 * 64 * UD : 0;
     static constexpr size_t LDS_R = (size_t)NW * RR * 4;
     static constexpr size_t LDS = LDS_Q + LDS_P + LDS_R + LDS_K;
-    static constexpr int OCC = NT > 1 || HD == 512 ? 2 : HD == 256 ? 3 : 4;   // waves per SIMD that the registers are held to
+    // Waves per SIMD that the registers are held to. (HD 256 with four row groups takes all 256 and spills one, which is written
+    // before the loop over the keys and read behind it.)
+    static constexpr int OCC = NT > 1 || HD == 512 ? 2 : HD == 256 ? 3 : 4;
 };
 
 constexpr float kv8_head = 6.f, kv8_move = 14.f;       // the reference lies 2^6 under its maximum and moves above 2^14
@@ -615,28 +621,32 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     if (tree || hr <= 64) {
         pl.nt = hr <= 16 ? 1 : hr <= 32 || HD == 512 ? 2 : 4;
         // Keys of a split, by the call's K and V in heads of 256 dims. Short ones leave a call to the prologues of its
-        // workgroups and the merge, long ones to the longest workgroup. 16 requests of 9K keys x 4 heads (576K) took 42.8 us
-        // in 256-key splits, 37.3 in 512 and 38.7 in 1024; of 32K keys (2M) 113.8 in 512 and 106.7 in 1024; 4 of 9K (144K)
-        // 19.7 in 256, 20.4 in 512 and 30.1 in 1024; one of 9K (36K) 13.0 in 128 and 15.2 in 256; 16 of up to 8K (524K) 25.7 in
-        // 256, 24.4 in 384 and 25.4 in 512, 8 of 9K (288K) 36.6, 32.7 and 36.1 (at HD 512
-        // 384 gains or loses by the lengths: 8 of up to 32K in two draws 26.0 and 30.4, 28.0 and 25.7 in 512). With more than 16 rows the
-        // partials weigh more: 16 trees of 48 rows over 16K keys (1M) 87.7 us in 512 and 72.8 in 1024. Up to four steps go
-        // without splits and their merge (9.5 us for 512 keys of 4 heads of 128, 10.4 in two splits).
+        // workgroups and the merge, long ones to the longest workgroup. us in 128 | 256 | 384 | 512 | 1024 keys, 24 q-heads over
+        // 4 of 256, K and V not in any cache: one request of 9K keys (36K) 16.8, 15.0, 16.5, 19.2, 28.2; 4 of 9K (144K) 28.7,
+        // 24.4, 22.0, 24.0, 29.4; 8 of 9K (288K) 45.6, 37.9, 33.2, 36.4, 36.0; 16 of up to 8K (524K) in three draws 33.1, 26.3,
+        // 25.0, 25.8, 30.6 | 28.1, 24.7, 22.7, 24.6, 29.8 | 28.0, 21.7, 21.9, 24.1, 30.1; 16 of 9K (576K) 74.4, 65.6, 60.1, 58.8,
+        // 59.6; 16 of 32K (2M) 239, 217, 199, 194, 182. At HD 512 8 of up to 32K in five draws 31.4 (geometric mean) in 256, 30.0
+        // in 384, 30.1 in 512. With more than 16 rows the partials weigh more: 16 trees of 48 rows over 16K keys (1M) 343,
+        // 208, 183, 161, 132; over up to 16K 165, 113, 101, 85.7, 65.9; 4 over 16K (256K) 87.3, 62.9, 59.0, 46.2, 52.0. Up to
+        // four steps go without splits and their merge: 256 keys 8.4 us, 11.2 in two splits (4 heads of 128), 9.8 and 11.5 (4 of
+        // 256); at 512 it is even at HD 128 (11.7, in four splits 11.2) and behind at HD 256 (14.8 and 12.3).
         const long long work = (long long)B * NKV * keys * HD / 256;
         if (chunk == 0) pl.C = work < 60000 ? 128 : work < 280000 ? 256 : work < 560000 && hr <= 16 && HD <= 256 ? 384 : work < (hr > 16 ? 700000 : 1500000) ? 512 : 1024;
         if (chunk == 0 && keys <= 512) pl.C = whole;
     } else {
         // Tiles of 64 rows. Where they do not fill the chip the split-KV form takes a prompt too: it walks 128 keys a step,
-        // and its row groups can be smaller and its keys split. Split-KV | tiles, us: causal 1400 x 16 q-heads over 8 (352
-        // tiles) 43.4 | 47.6, 1024 x 24 over 4 (384) 42.9 | 39.2, 800 x 24 behind 2000 (300) 112.6 | 85.8, 1000 x 16 over 8
-        // behind 2000 (250) 75.8 | 79.0; behind a window of 1024 500 x 16 over 8 (125) 35.2 | 38.2, 600 (150) 41.9 | 38.8; HD 512
-        // 800 x 16 (200) 42.7 | 46.7, 1024 (256) 57.1 | 54.2.
+        // and its row groups can be smaller and its keys split. Best split-KV | tiles, us: causal 1400 x 16 q-heads over 8 (352
+        // tiles) 41.5 | 46.9, 1500 (376) 46.9 | 50.5, 1024 x 24 over 4 (384) 38.9 | 38.9, 800 x 24 behind 2000 (300) 95.4 | 85.9, 1000
+        // x 16 over 8 behind 2000 (250) 76.5 | 79.3; behind a window of 1024 500 x 16 over 8 (125) 30.9 | 38.9, 600 (150) 37.1 | 39.3;
+        // HD 512 800 x 16 (200) 38.7 | 47.0, 1024 (256) 49.5 | 55.6, 1500 (375) 92.3 | 77.3.
         const long long n64 = std::min((long long)B * ((hr + 63) / 64), (long long)rows * G / 64 + B) * NKV;
         pl.tile = n64 >= (HD == 512 ? 250 : window > 0 && window <= max_pos ? 140 : keys <= 2304 ? 360 : 280) ? 64 : 0;
         if (!pl.tile) {
-            // 200 x 16 q-heads over 8 without a prefix: groups of 16 rows 9.5 us, 32 12.2, 64 16.9; 1000 behind 1000: 72, 53 and
-            // 64; 512 behind 4096: 64 rows in 1536-key splits 74, in 1024 87, no split of 16 rows 93. Fewer workgroups at HD
-            // 512: 500 x 16 over 1 behind 4000 117 us unsplit, 138 in 1536; 100 behind 4000 41 in 1024, 52 in 512.
+            // 200 x 16 q-heads over 8 without a prefix: groups of 16 rows 10.7 us, 32 13.4, 64 18.4; 1000 behind 1000: 74, 56 and
+            // 66; 512 behind 4096: 64 rows in 1152-key splits 65, in 1536 72, in 1024 93, no split of 16 rows 93. Fewer workgroups
+            // at HD 512: 500 x 16 over 1 behind 4000 113 us unsplit, 141 in 1536; 100 behind 4000 42 in 1024, 52 in 1536, 53 in 512,
+            // 104 unsplit. (Groups of 16 or 32 rows for keys of 900 to 1280 are close: 1024 x 16 over 8 31.3 and 32.0, 900 x 24 over
+            // 4 37.7 and 33.2, HD 512 800 x 16 43.2 and 38.7.)
             const long long n = HD == 512 ? n64 * 2 : n64, want = HD == 512 ? 200 : 450;
             pl.nt = HD == 512 ? 2 : 4;
             if (chunk == 0 && keys <= 1280) pl.nt = 1, pl.C = whole;
@@ -656,8 +666,12 @@ Kv8Plan kv8_choose(int B, int T, int rows, int NQ, int NKV, int HD, int max_pos,
     if (!pl.tile) return pl;
     if (pl.ns == 1) pl.C = 0;
     // Tiles of 128 rows where there are two rounds of them for the 512 workgroups that run at once (one, under a window: its
-    // tiles are equally long), else of 64. HD 256, us of 128 | 64 rows: 6 requests of up to 2500 x 24 q-heads over 4 (1400 tiles
-    // of 128) 326 | 361, 4096 behind a window of 1024, 16 over 8 (512) 79.7 | 87.9, causal 4096 of those (512) 202 | 153.
+    // tiles are equally long), else of 64. us of 128 | 64 rows, with the number of the former; HD 256: 6 requests of up to 2500
+    // x 24 q-heads over 4 (1330) 331 | 364, other lengths (880) 193 | 216; causal 4096, 16 over 8 (512) 208 | 155, 24 over 4 (768)
+    // 225 | 233, 8192 (1024) 524 | 551, two of 4096 (1024) 280 | 309; behind a window of 1024 3000 (375) 77 | 77, 3600 (450) 80 |
+    // 83, 4096 (512) 84 | 90, 6000 (750) 137 | 130, 4096 x 24 (768) 135 | 128, behind 512 4096 (512) 56 | 66: best where the rounds
+    // are whole. HD 128, 16 over 4: 2 of 2000 (500) 96 | 63, 8 of 1000 (1000) 63 | 69, 4 of 2000 (1000) 100 | 102, one of 8000 (1000)
+    // 345 | 300, 4 of 3000 (1500) 191 | 199.
     const long long all = std::min((long long)B * T, (long long)rows) * NQ * pl.ns;
     if (HD < 512 && all >= 128 * (window > 0 && window < max_pos ? 500 : 960)) pl.tile = 128;
     return pl;

@@ -501,11 +501,13 @@ template <int HD, class Cf> static hipError_t launch_pre(const Kv8PrefArgs &a, h
 
 hipError_t launch_kv8_prefill(const Kv8Problem &p, const Kv8Partials &part, const Kv8Plan &pl, hipStream_t st) {
     const Kv8PrefArgs a{p, part, part.C ? div_magic(part.C) : 0u, pl.ns, p.scale * kLog2e};
+    // (128 rows at HD 256 take all 256 registers and spill three; one of them is read again at the V loads of every step, a wait for
+    // the step's K loads with it.)
     const bool wide = pl.tile == 128;
     switch (p.c.HD) {
     case 128: return wide ? launch_pre<128, Kv8PrefCfg<128, 2, 4, 1, 2, 2>>(a, st) : launch_pre<128, Kv8PrefCfg<128, 2, 2, 2, 1, 3>>(a, st);
     case 256: return wide ? launch_pre<256, Kv8PrefCfg<256, 2, 4, 1, 2, 2>>(a, st) : launch_pre<256, Kv8PrefCfg<256, 2, 2, 2, 1, 2>>(a, st);
-    case 512:                                                          // (64 rows in 8 waves; before later steps 4 of 1500 x 16 q-heads 299 us, in 4 waves 333, 32 rows 444; 275 now)
+    case 512:                                                          // (64 rows in 8 waves; before later steps 4 of 1500 x 16 q-heads 299 us, in 4 waves 333, 32 rows 444; 277 now)
         return launch_pre<512, Kv8PrefCfg<512, 1, 4, 2, 1, 2>>(a, st);
     default: return hipErrorInvalidValue;
     }

@@ -144,7 +144,9 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
                            int *status, hipStream_t st) {
     const PlanArgs a{ctx, add, free_pages, free_in, table, free_out, cu, slots, status, table_stride, B, lp, cols, rows, free_cap};
     const int grid = free_in == free_out || rows <= 2048 ? 1 : (int)std::min(128ll, (rows + 2047ll) / 2048);
-    const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;     // fewer waves meet sooner at the barriers (4.5 us a call, 5.1 with 1024)
+    // Fewer waves meet sooner at the barriers: 16 requests of a token 2.9 us in 256 threads, 3.5 in 1024 (one after another in a
+    // graph), 256 of a token 3.3 and 4.0; 256 of four tokens take several rounds of rows, 6.0 and 4.2.
+    const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;
     if (rows <= kNarrow && cols <= kNarrow) hipLaunchKernelGGL(kv8_plan_kernel<int>, dim3(grid), dim3(threads), 0, st, a);
     else hipLaunchKernelGGL(kv8_plan_kernel<long long>, dim3(grid), dim3(threads), 0, st, a);
     return hipGetLastError();
@@ -162,8 +164,9 @@ hipError_t launch_kv8_plan(const int *ctx, const int *add, int B, int lp, int *t
 // A token with a value that is not finite gets K codes NaN and 0 in place of V's values that are not finite: a score with it
 // is NaN, so every row that attends it comes out NaN, and rows that do not are left alone (a NaN code in V would reach the
 // other rows of a matrix tile through 0 * NaN).
-// Bound by memory: 66K rows x 8 heads x 256 from bf16 read 2 bytes and write 1 per element, 172 us, 4.74 TB/s (a large copy
-// reaches 4.82). Small calls by latency: 16 rows of a token each 5.4 us, a prompt of 1024 from fp32 9.8.
+// Bound by memory: 66K rows x 8 heads x 256 from bf16 read 2 bytes and write 1 per element, 173 us, 4.73 TB/s (a large copy
+// reaches 4.82). Small calls by latency: 16 rows of a token each 5.2 us, a prompt of 1024 from fp32 8.8 (128 workgroups, one of
+// each run and head, on half of the CUs: its chain of load, maximum, transpose and store).
 struct AppendArgs {
     const void *k, *v;
     long ks, vs;                      // row strides in elements
@@ -438,9 +441,9 @@ hipError_t launch_kv8_append(const void *k, const void *v, int src_dtype, long k
     AppendArgs a{k, v, k_stride, v_stride, c, slots, stats, rows, 1, 0, 0};
     while ((8 << a.lv) < c.HD) a.lv++;
     // A workgroup looks for runs among `win` rows, and takes those that begin there one after another. Windows of 1 | 4 | 16
-    // rows, us: 16 requests of a token x 4 heads (64 units) 5.9 | 13.8 | 45.9, 256 of a token x 4 (1024) 13.6 | 16.2 | 46.0, 512
-    // of up to 4 x 8 (10K) 58.7 | 50.1 | 62.6, a prompt of 1024 x 8 (8K) 15.6 | 12.1 | 15.6, 66K rows of prompts x 8 (532K) 364 |
-    // 211 | 172: most workgroups of a prompt find none.
+    // rows, us: 16 requests of a token x 4 heads (64 units) 5.2 | 13.3 | 46.1, 256 of a token x 4 (1024) 13.1 | 15.8 | 46.7, 512
+    // of up to 4 x 8 (10K) 56.8 | 49.6 | 60.0, a prompt of 1024 x 8 (8K) from bf16 11.4 | 7.5 | 8.3, from fp32 16.7 | 8.7 | 7.4, 66K rows
+    // of prompts x 8 (532K) 383 | 212 | 165: most workgroups of a prompt find none.
     const long long units = (long long)rows * c.NKV;
     a.win = units <= 4096 ? 1 : units <= 32768 ? 4 : 16;
     a.windows = (rows - 1) / a.win + 1;
