@@ -712,6 +712,7 @@ size_t dgx_attn_kv8_workspace(int B, int T, int rows, int NQ, int NKV, int HD, i
     if (!kv8_sizes_ok(B, T, rows, NQ, NKV, HD, max_pos, chunk)) return (size_t)-1;
     if (B == 0 || T == 0 || rows == 0) return 0;
     if (window < 0) window = 0;
+    T = std::min(T, rows);
     int ns = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, tree != 0).ns;
     if (!tree && T <= 32) ns = std::max(ns, kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window, true).ns);
     if (ns > 1 && !kv8_partials_ok(rows, NQ, ns)) return (size_t)-1;
@@ -722,7 +723,7 @@ hipError_t dgx_attn_kv8_form(int B, int T, int rows, int NQ, int NKV, int HD, in
     if (!form || !kv8_sizes_ok(B, T, rows, NQ, NKV, HD, max_pos, chunk)) return hipErrorInvalidValue;
     for (int i = 0; i < 4; i++) form[i] = 0;
     if (B == 0 || T == 0 || rows == 0) return hipSuccess;
-    const Kv8Plan pl = kv8_choose(B, T, rows, NQ, NKV, HD, max_pos, chunk, window < 0 ? 0 : window, tree != 0);
+    const Kv8Plan pl = kv8_choose(B, std::min(T, rows), rows, NQ, NKV, HD, max_pos, chunk, window < 0 ? 0 : window, tree != 0);
     form[0] = pl.tile;
     form[1] = pl.tile ? pl.tile : 16 * pl.nt;
     form[2] = pl.C;
@@ -742,6 +743,7 @@ hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const 
         (!cu && rows != B * T) || (anc && T > 32))
         return hipErrorInvalidValue;
     if (window < 0) window = 0;
+    T = std::min(T, rows);                                             // (a request has no more: a bound far past them must not size the grid)
     const Kv8Problem p{c, Q, q_dtype, O, o_dtype, lse, B, T, rows, NQ, ctx, cu, table, table_stride,
                        reinterpret_cast<const uint32_t *>(anc), max_pos, resolve_scale(scale, c.HD), window};
     const Kv8Plan pl = kv8_choose(B, T, rows, NQ, c.NKV, c.HD, max_pos, chunk, window, anc != nullptr);

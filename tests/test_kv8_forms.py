@@ -73,3 +73,12 @@ def test_the_device_check_without_the_raw_getter(monkeypatch):
     for dev in (0, -1):
         with pytest.raises(ValueError):
             A._here(dev, "attn_kv8")
+
+
+def test_a_bound_past_the_rows_is_the_rows():
+    """T bounds a request's rows, which are no more than all rows: the form and the workspace are those of the smaller one."""
+    for T in (6, 100, 1 << 26):
+        for window, chunk in ((0, 0), (100, 64)):
+            args = (2, 5, 24, 4, 256, 9000, chunk, window)
+            assert A.attn_kv8_form(2, T, *args[1:]) == A.attn_kv8_form(2, 5, *args[1:])
+            assert A.attn_kv8_workspace(2, T, *args[1:]) == A.attn_kv8_workspace(2, 5, *args[1:])
