@@ -54,3 +54,11 @@ def attend(heads, page, ctx, add, T, mp, shift=0, window=0, chunk=0):
 def test_a_bound_on_a_requests_rows_far_past_them(T, window):
     attend((24, 4, 256), 64, [100, 0, 300], [1, 3, 1], T, 400, window=window)
     attend((16, 1, 512), 16, [100, 0], [1, 70], min(T, 1 << 25), 400, window=window, chunk=64)
+
+
+@pytest.mark.parametrize("heads,add,chunk", [((8, 2, 128), [1, 1], 0), ((8, 2, 128), [1, 1], 64), ((16, 1, 512), [8, 3], 128), ((4, 2, 256), [90, 1], 64),
+                                             ((4, 2, 256), [90, 1], 0), ((64, 32, 256), [90, 70], 0), ((64, 32, 256), [90, 70], 64)])
+def test_the_last_positions(heads, add, chunk):
+    """Windows that end at position 2^30 - 1, the largest max_pos."""
+    shift = (1 << 30) - 1024
+    attend(heads, 64, [1024 - add[0], 700], add, max(add), (1 << 30) - 1, shift, window=200, chunk=chunk)
