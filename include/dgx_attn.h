@@ -273,7 +273,8 @@ hipError_t dgx_kv8_append(const void *k_src, const void *v_src, int src_dtype, l
  * chunk: keys of a split (a multiple of 64; 0: chosen from the sizes). ws: dgx_attn_kv8_workspace bytes for the same
  * sizes, 16-byte aligned, used by this call alone until it has run (calls on other streams and other graphs take their
  * own). Results do not depend on the other requests of a batch, but the forms chosen from B, T, rows and max_pos do.
- * hipErrorInvalidValue for sizes or types outside the above, or a workspace that is too small. */
+ * hipErrorInvalidValue for sizes or types outside the above or past max_pos < 2^30, chunk <= 2^20, NQ <= 65535, B * T < 2^31 and
+ * T * NQ / NKV < 2^30, or a workspace that is too small. */
 hipError_t dgx_attn_kv8(const void *Q, int q_dtype, const dgx_kv8 *cache, const int *table, long table_stride, void *O, int o_dtype,
                         float *lse, int B, int T, int rows, int NQ, const int *ctx, const int *cu, const unsigned *anc, int max_pos,
                         int chunk, void *ws, size_t ws_bytes, hipStream_t st, float scale, int window);
